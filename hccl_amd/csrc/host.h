@@ -46,9 +46,16 @@ HcclResult CheckReduceOp(HcclDataType t, HcclReduceOp op);
 // ---------------------------------------------------------------------------------------------
 enum class OpType {
     ALL_REDUCE, REDUCE_SCATTER, ALL_GATHER, ALL_GATHER_V, ALL_TO_ALL_V,
-    REDUCE_SCATTER_V, REDUCE, BROADCAST, SCATTER, BARRIER
+    REDUCE_SCATTER_V, REDUCE, BROADCAST, SCATTER, BARRIER,
+    TOKEN_LOG_PROBS, GRAD_NORM   // collectives of another library over the same worlds: see LaunchFn
 };
 const char* OpName(OpType t);
+
+struct World;
+struct PendingOp;
+// What the call that completes a set runs for a collective whose kernels live in another library (include/
+// hccl_model_ops.h): everything that library needs of a rank's call travels in RankArgs::var.
+typedef HcclResult (*LaunchFn)(World* w, PendingOp& p, hipStream_t s);
 
 struct RankArgs {
     const void* send = nullptr;
@@ -70,6 +77,7 @@ struct PendingOp {
     bool done = false;
     HcclResult result = HCCL_SUCCESS;
     bool noAlloc = false;   // the allocation-free variant of the entry point was called
+    LaunchFn launch = nullptr;   // null: one of this library's own operators, by `type`
     std::vector<RankArgs> ranks;
 };
 
@@ -106,7 +114,6 @@ struct CopySeg {
     uint64_t len;
 };
 
-struct World;
 struct Comm {
     uint32_t magic = kMagic;
     World* world = nullptr;
@@ -283,7 +290,8 @@ struct DeviceScope {
 // Deposits one rank's arguments of a collective; the call that completes the set launches.  Blocks until the set
 // is complete outside a group (HcclGroupStart / End), returns at once inside one.
 HcclResult Submit(const CommRef& ref, OpType type, HcclDataType dtype, HcclReduceOp op, uint64_t count, const void* send,
-                  void* recv, hipStream_t stream, std::vector<uint64_t>&& var, uint32_t root = 0, bool noAlloc = false);
+                  void* recv, hipStream_t stream, std::vector<uint64_t>&& var, uint32_t root = 0, bool noAlloc = false,
+                  LaunchFn launch = nullptr);
 // A call that fails its argument checks after its communicator has been identified still takes its place in
 // the rank's sequence of collectives: the peers of that collective wake at once with the same verdict (nothing
 // is launched), and the calls that follow pair up as they would have.

@@ -130,6 +130,8 @@ const char* OpName(OpType t)
         case OpType::BROADCAST: return "Broadcast";
         case OpType::SCATTER: return "Scatter";
         case OpType::BARRIER: return "Barrier";
+        case OpType::TOKEN_LOG_PROBS: return "TokenLogProbs";
+        case OpType::GRAD_NORM: return "GradNorm";
         default: return "AlltoAllV";
     }
 }

@@ -1,0 +1,131 @@
+// Launch descriptors of the model operators (include/hccl_model_ops.h), shared by their host layer and their kernels.
+// Plain data that travels in the kernel-argument segment, below 4 KiB each.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "hccl_model_ops.h"
+
+namespace hccl_amd {
+namespace model_ops {
+
+constexpr uint32_t kMaxShards = HCCL_AMD_MAX_RANKS;
+constexpr uint32_t kMaxTop = HCCL_AMD_MAX_TOP;
+
+// ---- log probabilities ----------------------------------------------------------------------------------------
+// One row of logits is the concatenation of nShards parts.
+struct LogProbsArgs {
+    const void* logits[kMaxShards];
+    uint64_t rowStride[kMaxShards];     // elements
+    uint32_t count[kMaxShards];         // elements of the part
+    const void* tokens;
+    float* stats;           // nSplit > 1: [row][split][4] = max, sum, weighted sum, -
+    uint64_t* keys;         //             [row][split][topCount], descending, 0 where there is none
+    uint32_t nShards;
+    uint32_t nSplit;        // workgroups per row
+    uint32_t vocab;
+    uint32_t topCount;
+    uint32_t wideTokens;    // tokens and topIds are 64-bit
+    float scale;
+    float exp2Scale;        // scale * log2(e)
+    uint32_t nOut;
+    struct Out {
+        float* logProbs;
+        float* logSumExp;
+        float* entropy;
+        float* topValues;
+        void* topIds;
+    } out[kMaxShards];
+};
+static_assert(sizeof(LogProbsArgs) <= 4096, "kernel arguments");
+
+// Workgroups per row, from the sizes alone.
+uint32_t LogProbsSplit(uint64_t rows, uint64_t vocab);
+inline uint64_t LogProbsWorkspace(uint64_t rows, uint64_t vocab, uint32_t top)
+{
+    const uint64_t split = LogProbsSplit(rows, vocab);
+    return split <= 1 ? 0 : rows * split * (4 * sizeof(float) + top * sizeof(uint64_t));
+}
+hipError_t LaunchLogProbs(const LogProbsArgs& args, HcclDataType dtype, uint32_t rows, hipStream_t stream);
+
+// ---- their gradient ---------------------------------------------------------------------------------------------
+struct LogProbsGradArgs {
+    const void* logits;
+    void* grad;
+    uint64_t rowStride;      // elements
+    uint64_t gradRowStride;
+    uint32_t vocabStart;
+    uint32_t count;
+    uint32_t topCount;
+    uint32_t wideTokens;
+    float scale;
+    const void* tokens;
+    const float* logSumExp;
+    const float* entropy;
+    const float* gradLogProbs;
+    const float* gradEntropy;
+    const void* topIds;
+    const float* gradTop;
+};
+hipError_t LaunchLogProbsGrad(const LogProbsGradArgs& args, HcclDataType dtype, uint32_t rows, hipStream_t stream);
+
+// ---- gradient norm ------------------------------------------------------------------------------------------------
+// A batch of tensors cut into chunks of kNormChunkBytes; workgroup b sums the chunks [b * perGroup, (b + 1) * perGroup).
+constexpr uint32_t kNormBatch = 240;            // tensors per launch
+constexpr uint32_t kNormGroups = 2048;          // partial sums per launch
+constexpr uint32_t kNormChunkBytes = 16384;
+struct NormArgs {
+    const void* data[kNormBatch];
+    uint32_t chunkEnd[kNormBatch];      // inclusive prefix of the chunk counts
+    uint32_t lastChunk[kNormBatch];     // elements of the tensor's last chunk, << 2 | type (0 fp32, 1 bf16, 2 fp16)
+    double* partial;                    // one per workgroup
+    uint32_t nTensors;
+    uint32_t nChunks;
+    uint32_t perGroup;
+};
+static_assert(sizeof(NormArgs) <= 4096, "kernel arguments");
+struct NormJoinArgs {
+    const double* partial;
+    uint32_t nPartial;
+    float maxNorm;
+    float scale;
+    uint32_t nOut;
+    float* out[kMaxShards];
+};
+hipError_t LaunchNormBatch(const NormArgs& args, uint32_t groups, hipStream_t stream);
+hipError_t LaunchNormJoin(const NormJoinArgs& args, hipStream_t stream);
+
+// ---- AdamW ----------------------------------------------------------------------------------------------------------
+constexpr uint32_t kAdamWBatch = 52;            // tensors per launch
+constexpr uint32_t kAdamWChunk = 4096;          // elements per workgroup, a multiple of the state block
+struct AdamWArgs {
+    struct Tensor {
+        void* param;
+        const void* grad;
+        void* m;
+        void* v;
+        float* master;
+        float* mScale;
+        float* vScale;
+        uint64_t count;
+    } t[kAdamWBatch];
+    uint32_t chunkEnd[kAdamWBatch];     // inclusive prefix of the chunk counts
+    uint32_t nTensors;
+    uint32_t skipNonFinite;
+    const float* clip;
+    const int64_t* step;                // null: the host's factors below
+    const float* lr;
+    float beta1, oneMinusBeta1, beta2, oneMinusBeta2;
+    float eps;
+    float weightDecay;
+    float hostLr;
+    float logBeta1, logBeta2;           // natural logarithms, for a step read on the device
+    float correction1, rootCorrection2; // 1 / (1 - beta1^step), 1 / sqrt(1 - beta2^step)
+};
+static_assert(sizeof(AdamWArgs) <= 4096, "kernel arguments");
+hipError_t LaunchAdamW(const AdamWArgs& args, HcclDataType paramType, HcclDataType gradType, bool master, bool fp8State,
+                       uint32_t chunks, hipStream_t stream);
+
+}  // namespace model_ops
+}  // namespace hccl_amd

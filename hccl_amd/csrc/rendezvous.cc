@@ -68,6 +68,8 @@ HcclResult Launch(World* w, PendingOp& p, uint32_t launcher)
     HcclResult rc;
     if (p.type == OpType::BARRIER) {
         rc = HCCL_SUCCESS;   // the ordering of the streams around this point is the whole operation
+    } else if (p.launch != nullptr) {
+        rc = p.launch(w, p, s);
     } else if (w->n == 1) {
         rc = RunSingleRank(w, p, s);
     } else {
@@ -118,7 +120,7 @@ void PopFinished(World* w)
 // The cell of rank `rank`'s next call in the world's sequence of collectives (created by the first rank to get
 // there).  Caller holds w->mu.
 std::shared_ptr<PendingOp> NextCell(World* w, uint32_t rank, OpType type, HcclDataType dtype, HcclReduceOp op,
-                                    uint64_t count, uint32_t root, bool noAlloc, bool* created)
+                                    uint64_t count, uint32_t root, bool noAlloc, LaunchFn launch, bool* created)
 {
     const uint64_t seq = w->nextSeq[rank]++;
     while (w->baseSeq + w->pending.size() <= seq) {
@@ -134,6 +136,7 @@ std::shared_ptr<PendingOp> NextCell(World* w, uint32_t rank, OpType type, HcclDa
         cell->count = count;
         cell->root = root;
         cell->noAlloc = noAlloc;
+        cell->launch = launch;
         cell->ranks.resize(w->n);
     }
     return cell;
@@ -141,7 +144,8 @@ std::shared_ptr<PendingOp> NextCell(World* w, uint32_t rank, OpType type, HcclDa
 
 // Deposits one rank's arguments; the call that completes the set launches.
 HcclResult Submit(const CommRef& ref, OpType type, HcclDataType dtype, HcclReduceOp op, uint64_t count, const void* send,
-                  void* recv, hipStream_t stream, std::vector<uint64_t>&& var, uint32_t root, bool noAlloc)
+                  void* recv, hipStream_t stream, std::vector<uint64_t>&& var, uint32_t root, bool noAlloc,
+                  LaunchFn launch)
 {
     Comm* c = ref.c;
     World* w = c->world;
@@ -151,7 +155,7 @@ HcclResult Submit(const CommRef& ref, OpType type, HcclDataType dtype, HcclReduc
         return HCCL_E_UNAVAIL;
     }
     bool created = false;
-    std::shared_ptr<PendingOp> p = NextCell(w, c->rank, type, dtype, op, count, root, noAlloc, &created);
+    std::shared_ptr<PendingOp> p = NextCell(w, c->rank, type, dtype, op, count, root, noAlloc, launch, &created);
     p->arrived++;
     if (p->done) {
         // Settled before this rank arrived: a peer's call failed its checks, or timed out.
@@ -160,7 +164,7 @@ HcclResult Submit(const CommRef& ref, OpType type, HcclDataType dtype, HcclReduc
         return rc;
     }
     if (p->type != type || p->dtype != dtype || p->op != op || p->count != count || p->root != root ||
-        p->noAlloc != noAlloc) {
+        p->noAlloc != noAlloc || p->launch != launch) {
         Log(1, "%s on rank %u does not match the call of the other ranks (%s, count %llu, type %d, root %u)",
             OpName(type), c->rank, OpName(p->type), (unsigned long long)p->count, static_cast<int>(p->dtype), p->root);
         p->result = HCCL_E_PARA;
@@ -221,7 +225,7 @@ HcclResult Reject(const CommRef& ref, OpType type, HcclResult rc)
     }
     bool created = false;
     std::shared_ptr<PendingOp> p = NextCell(w, ref.c->rank, type, HCCL_DATA_TYPE_RESERVED, HCCL_REDUCE_RESERVED, 0, 0,
-                                            false, &created);
+                                            false, nullptr, &created);
     p->arrived++;
     if (!p->done) {
         if (p->result == HCCL_SUCCESS) {

@@ -1,0 +1,182 @@
+"""ctypes view of libhccl_amd_model_ops.so (include/hccl_model_ops.h): the operators a training or serving step runs next
+to its collectives, over the communicators of this package.
+
+* :func:`token_log_probs` -- log probabilities of given tokens, entropy and top alternatives over a vocabulary that is
+  split across the ranks; a collective, every rank receives the results.
+* :func:`token_log_probs_grad` -- its gradient with respect to one rank's part of the logits.
+* :func:`grad_norm` -- 2-norm over all gradient tensors of all ranks and the factor that clips it; a collective.
+* :func:`adamw` -- one AdamW step over many tensors, with states in 32 bits or in FP8 blocks of 256 elements.
+
+Buffers are device pointers (integers, ctypes pointers or anything with ``data_ptr()``), counts are elements, ``stream``
+must not be null, and a failing call raises :class:`hccl_amd.HcclError`, as for the collectives.  Drive several ranks from
+one thread inside ``with hccl_amd.group():``.  What the arguments mean is written in the header.
+"""
+import ctypes
+import os
+
+import hccl_amd
+from hccl_amd import HcclDataType, _as_ptr, _as_stream, check
+
+_HERE = os.path.dirname(os.path.abspath(__file__))
+LIB_PATH = os.path.join(_HERE, "libhccl_amd_model_ops.so")
+MAX_TOP = 32
+STATE_BLOCK = 256
+
+_vp, _u64, _u32, _i32, _f32, _f64 = (ctypes.c_void_p, ctypes.c_uint64, ctypes.c_uint32, ctypes.c_int, ctypes.c_float,
+                                     ctypes.c_double)
+
+
+class TokenLogProbsArgs(ctypes.Structure):
+    """HcclAmdTokenLogProbsArgs."""
+    _fields_ = [("logits", _vp), ("rowStride", _u64), ("vocabStart", _u64), ("vocabCount", _u64), ("tokenCount", _u64),
+                ("tokens", _vp), ("dataType", _i32), ("tokenType", _i32), ("scale", _f32), ("topCount", _u32),
+                ("logProbs", _vp), ("logSumExp", _vp), ("entropy", _vp), ("topValues", _vp), ("topIds", _vp),
+                ("workspace", _vp), ("workspaceBytes", _u64)]
+
+
+class TokenLogProbsGradArgs(ctypes.Structure):
+    """HcclAmdTokenLogProbsGradArgs."""
+    _fields_ = [("logits", _vp), ("rowStride", _u64), ("vocabStart", _u64), ("vocabCount", _u64), ("tokenCount", _u64),
+                ("tokens", _vp), ("dataType", _i32), ("tokenType", _i32), ("scale", _f32), ("topCount", _u32),
+                ("logSumExp", _vp), ("entropy", _vp), ("gradLogProbs", _vp), ("gradEntropy", _vp), ("topIds", _vp),
+                ("gradTopValues", _vp), ("gradLogits", _vp), ("gradRowStride", _u64)]
+
+
+class NormTensor(ctypes.Structure):
+    """HcclAmdNormTensor."""
+    _fields_ = [("data", _vp), ("count", _u64), ("dataType", _i32)]
+
+
+class AdamWTensor(ctypes.Structure):
+    """HcclAmdAdamWTensor."""
+    _fields_ = [("param", _vp), ("grad", _vp), ("expAvg", _vp), ("expAvgSq", _vp), ("master", _vp), ("expAvgScale", _vp),
+                ("expAvgSqScale", _vp), ("count", _u64), ("paramType", _i32), ("gradType", _i32)]
+
+
+class AdamWConfig(ctypes.Structure):
+    """HcclAmdAdamWConfig."""
+    _fields_ = [("lr", _f64), ("beta1", _f64), ("beta2", _f64), ("eps", _f64), ("weightDecay", _f64), ("step", _u64),
+                ("stepOnDevice", _vp), ("lrOnDevice", _vp), ("clip", _vp), ("stateType", _i32), ("skipNonFinite", _i32)]
+
+
+_lib = None
+
+
+def lib():
+    """Loads libhccl_amd_model_ops.so; raises if it has not been built."""
+    global _lib
+    if _lib is not None:
+        return _lib
+    hccl_amd.lib()      # the library it works on
+    if not os.path.exists(LIB_PATH):
+        raise ImportError("%s is missing: run `make -C hccl_amd/csrc` (or hccl_amd.build()) first" % LIB_PATH)
+    _lib = _bind(ctypes.CDLL(LIB_PATH))
+    return _lib
+
+
+def _bind(L):
+    """Declares the argument and result types of the library's entry points on the loaded library L."""
+    L.HcclAmdTokenLogProbs.argtypes = [ctypes.POINTER(TokenLogProbsArgs), _vp, _vp]
+    L.HcclAmdTokenLogProbsWorkspace.argtypes = [_u64, _u64, _u32, ctypes.POINTER(_u64)]
+    L.HcclAmdTokenLogProbsGrad.argtypes = [ctypes.POINTER(TokenLogProbsGradArgs), _vp, _vp]
+    L.HcclAmdGradNorm.argtypes = [ctypes.POINTER(NormTensor), _u32, _f32, _f32, _vp, _vp, _u64, _vp, _vp]
+    L.HcclAmdGradNormWorkspace.argtypes = [_u64, ctypes.POINTER(_u64)]
+    L.HcclAmdAdamW.argtypes = [ctypes.POINTER(AdamWTensor), _u32, ctypes.POINTER(AdamWConfig), _vp, _vp]
+    for name in ("HcclAmdTokenLogProbs", "HcclAmdTokenLogProbsWorkspace", "HcclAmdTokenLogProbsGrad", "HcclAmdGradNorm",
+                 "HcclAmdGradNormWorkspace", "HcclAmdAdamW"):
+        getattr(L, name).restype = ctypes.c_int
+    return L
+
+
+def _address(buf):
+    """_as_ptr as a structure's field takes it."""
+    if buf is None or isinstance(buf, int):
+        return buf
+    if hasattr(buf, "data_ptr"):
+        return buf.data_ptr()
+    return _as_ptr(buf).value
+
+
+def token_log_probs_workspace(token_count, vocab_size, top_count=0):
+    """Bytes of workspace a token_log_probs call over `token_count` rows of `vocab_size` entries (all ranks') needs."""
+    size = ctypes.c_uint64()
+    check(lib().HcclAmdTokenLogProbsWorkspace(token_count, vocab_size, top_count, ctypes.byref(size)),
+          "HcclAmdTokenLogProbsWorkspace")
+    return size.value
+
+
+def token_log_probs(hccl_comm, logits, token_count, vocab_start, vocab_count, tokens, log_probs,
+                    data_type=HcclDataType.BFP16, token_type=HcclDataType.INT64, row_stride=None, scale=1.0, lse=None,
+                    entropy=None, top_count=0, top_values=None, top_ids=None, workspace=None, workspace_bytes=0,
+                    stream=None):
+    """Log probabilities of `tokens` under softmax(scale * logits), whose columns vocab_start .. vocab_start + vocab_count
+    this rank holds; every output (log_probs, lse, entropy, top_values, top_ids) may be None."""
+    args = TokenLogProbsArgs(_address(logits), vocab_count if row_stride is None else row_stride, vocab_start, vocab_count,
+                             token_count, _address(tokens), data_type, token_type, scale, top_count, _address(log_probs),
+                             _address(lse), _address(entropy), _address(top_values), _address(top_ids),
+                             _address(workspace), workspace_bytes)
+    return check(lib().HcclAmdTokenLogProbs(args, hccl_comm, _as_stream(stream)), "HcclAmdTokenLogProbs")
+
+
+def token_log_probs_grad(hccl_comm, logits, token_count, vocab_start, vocab_count, tokens, lse, grad_log_probs, grad_logits,
+                         data_type=HcclDataType.BFP16, token_type=HcclDataType.INT64, row_stride=None,
+                         grad_row_stride=None, scale=1.0, entropy=None, grad_entropy=None, top_count=0, top_ids=None,
+                         grad_top_values=None, stream=None):
+    """Writes the gradient with respect to this rank's part of the logits to `grad_logits` (which may be the logits
+    themselves); local to the rank."""
+    args = TokenLogProbsGradArgs(_address(logits), vocab_count if row_stride is None else row_stride, vocab_start,
+                                 vocab_count, token_count, _address(tokens), data_type, token_type, scale, top_count,
+                                 _address(lse), _address(entropy), _address(grad_log_probs), _address(grad_entropy),
+                                 _address(top_ids), _address(grad_top_values), _address(grad_logits),
+                                 vocab_count if grad_row_stride is None else grad_row_stride)
+    return check(lib().HcclAmdTokenLogProbsGrad(args, hccl_comm, _as_stream(stream)), "HcclAmdTokenLogProbsGrad")
+
+
+def norm_tensors(tensors):
+    """The array grad_norm takes, from (buffer, count, data type) triples; it can be kept while the buffers stay."""
+    items = [NormTensor(_address(buf), count, int(data_type)) for buf, count, data_type in tensors]
+    return (NormTensor * len(items))(*items)
+
+
+def grad_norm_workspace(tensor_count):
+    """Bytes of workspace a grad_norm call over `tensor_count` tensors, all ranks' together, needs."""
+    size = ctypes.c_uint64()
+    check(lib().HcclAmdGradNormWorkspace(tensor_count, ctypes.byref(size)), "HcclAmdGradNormWorkspace")
+    return size.value
+
+
+def grad_norm(hccl_comm, tensors, max_norm, result, scale=1.0, workspace=None, workspace_bytes=0, stream=None):
+    """result[0] = |scale| * 2-norm of all tensors of all ranks, result[1] = scale * the factor that brings it to
+    `max_norm` (max_norm <= 0: no clipping).  `tensors`: what norm_tensors returned, or its argument."""
+    if not isinstance(tensors, ctypes.Array):
+        tensors = norm_tensors(tensors)
+    return check(lib().HcclAmdGradNorm(tensors, len(tensors), max_norm, scale, _as_ptr(result), _as_ptr(workspace),
+                                       workspace_bytes, hccl_comm, _as_stream(stream)), "HcclAmdGradNorm")
+
+
+def adamw_tensors(tensors):
+    """The array adamw takes, from dicts with param, grad, exp_avg, exp_avg_sq, count, param_type, grad_type and, where
+    they are wanted, master, exp_avg_scale, exp_avg_sq_scale; it can be kept while the buffers stay."""
+    items = []
+    for t in tensors:
+        unknown = set(t) - {"param", "grad", "exp_avg", "exp_avg_sq", "master", "exp_avg_scale", "exp_avg_sq_scale",
+                            "count", "param_type", "grad_type"}
+        if unknown:
+            raise TypeError("adamw_tensors: unknown fields %s" % sorted(unknown))
+        items.append(AdamWTensor(_address(t["param"]), _address(t["grad"]), _address(t["exp_avg"]),
+                                 _address(t["exp_avg_sq"]), _address(t.get("master")), _address(t.get("exp_avg_scale")),
+                                 _address(t.get("exp_avg_sq_scale")), t["count"], int(t["param_type"]),
+                                 int(t["grad_type"])))
+    return (AdamWTensor * len(items))(*items)
+
+
+def adamw(hccl_comm, tensors, step, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01,
+          state_type=HcclDataType.FP32, clip=None, skip_non_finite=False, step_on_device=None, lr_on_device=None,
+          stream=None):
+    """One AdamW step over all `tensors` (what adamw_tensors returned, or its argument); local to the rank.  `clip` is a
+    grad_norm result; `step` counts from 1 (step_on_device: an int64 on the device that is read instead)."""
+    if not isinstance(tensors, ctypes.Array):
+        tensors = adamw_tensors(tensors)
+    config = AdamWConfig(lr, beta1, beta2, eps, weight_decay, step, _address(step_on_device), _address(lr_on_device),
+                         _address(clip), int(state_type), 1 if skip_non_finite else 0)
+    return check(lib().HcclAmdAdamW(tensors, len(tensors), config, hccl_comm, _as_stream(stream)), "HcclAmdAdamW")
