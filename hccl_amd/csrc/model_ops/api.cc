@@ -95,7 +95,7 @@ HcclResult RunTokenLogProbs(World* w, PendingOp& p, hipStream_t s)
 {
     LogProbsArgs a = {};
     const uint64_t rows = p.count;
-    uint64_t vocab = 0;
+    uint64_t vocab = 0, vectors = 0;
     std::vector<HcclAmdTokenLogProbsArgs> ranks(w->n);
     for (uint32_t r = 0; r < w->n; ++r) {
         ranks[r] = FromWords<HcclAmdTokenLogProbsArgs>(p.ranks[r].var);
@@ -111,6 +111,7 @@ HcclResult RunTokenLogProbs(World* w, PendingOp& p, hipStream_t s)
             a.logits[a.nShards] = x.logits;
             a.rowStride[a.nShards] = x.rowStride;
             a.count[a.nShards] = static_cast<uint32_t>(x.vocabCount);
+            vectors += LogProbsVectors(x.vocabCount, DataTypeSize(p.dtype));
             a.nShards++;
         }
         if (a.tokens == nullptr) {
@@ -134,7 +135,8 @@ HcclResult RunTokenLogProbs(World* w, PendingOp& p, hipStream_t s)
     a.wideTokens = ranks[0].tokenType == HCCL_DATA_TYPE_INT64 ? 1 : 0;
     a.scale = ranks[0].scale;
     a.exp2Scale = static_cast<float>(static_cast<double>(a.scale) * 1.4426950408889634);
-    a.nSplit = LogProbsSplit(rows, vocab);
+    a.vectors = static_cast<uint32_t>(vectors);
+    a.nSplit = LogProbsFormOf(rows, vectors).split;
     if (a.nSplit > 1) {
         const uint64_t need = LogProbsWorkspace(rows, vocab, top);
         void* space = nullptr;

@@ -1,19 +1,25 @@
 // Log probabilities of given tokens, entropy and top alternatives of rows of logits whose vocabulary lies in up to 64
 // parts (one per rank).
 //
-// With x = scale * logit, one pass over a row keeps, per lane, the largest logit m, s = sum exp(x - scale m) and
-// t = sum y exp2(y), y = log2(e) (x - scale m): whenever m grows, s and t are carried over to the new reference,
-// s' = s c, t' = c (t + s d), c = exp2(d), d = log2(e) scale (m - m').  Differences to the maximum are formed before they
-// are scaled, so that rows of the type's lowest value (a mask) come out like any other row of equal logits.
-//   lse = scale m + ln s, entropy = ln s - ln 2 t / s.
+// One pass over a row keeps, per lane, the largest logit, a reference m = c * largest (c = scale * log2 e, no lower than
+// -2^20), s = sum exp2(y) and t = sum y exp2(y) with y = c x - m in one multiply-add.  Whenever m grows, both are carried
+// over: d = m - m', s' = s 2^d, t' = 2^d (t + s d).  Then
+//   lse = ln 2 (m + log2 s), log p = ln 2 (y - log2 s), entropy = ln 2 (log2 s - t / s),
+// in which the rounding of m cancels.  That holds while |m| stays small against 2^24; a row whose largest logit lies beyond
+// (lowest values as masks, infinities) is read once more with y = c (x - largest), where nothing but the difference is
+// scaled.
 //
-// Alternatives without a second pass: the k-th largest of the 256 lane maxima bounds the k-th largest element of the row
-// from below, since k lanes hold an element at least as large.  Only lanes whose maximum reaches the bound can hold one of
-// the k, so their elements alone (k / 256 of the row, still in the cache) are looked at again; what reaches the bound is
-// ranked by (logit, lower index).  Rows with so many equal logits that the list overflows are searched exactly instead.
+// Alternatives without a second pass over the row: a histogram of the lane maxima, by their distance from the largest,
+// yields a bound that topCount lanes reach, and so topCount elements.  Every lane also leaves the largest of each group of
+// vectors it loads together in LDS (16 bits of its order), and only groups that reach the bound are read again: four
+// vectors for each of the topCount and a few more, instead of the row, which no cache holds any longer.  What reaches the
+// bound is ranked by (logit, lower index).  Where too many reach it (equal logits, as in a row that a mask leaves few entries
+// of), the exact topCount-th lane maximum takes its place: what lies above is in fewer than topCount lanes, and the rest are
+// the first entries equal to it.
 //
-// Bound: one read of the logits from HBM.  Every workgroup owns one row; where there are few rows, nSplit workgroups share
-// each and a second kernel joins their partial results.
+// Bound: one read of the logits from HBM, closely followed by the vector ALU (about eight instructions and an exponential,
+// which takes two slots, per element).  A workgroup owns one row; where there are few rows, nSplit workgroups share each and
+// a second kernel joins their partial results.
 #include "model_ops.h"
 #include "vec.h"
 
@@ -21,13 +27,15 @@ namespace hccl_amd {
 namespace model_ops {
 namespace {
 
-constexpr uint32_t kThreads = 256;
-constexpr uint32_t kWaves = kThreads / kWave;
 constexpr uint32_t kUnroll = 4;            // vectors a lane loads together
-constexpr uint32_t kCandidates = 1024;     // elements of a row that may reach the bound before the exact search takes over
+// Elements, and groups, that may reach the bound before the exact search takes over.
+template <uint32_t kThreads>
+constexpr uint32_t kCandidates = kThreads == kWave ? 256 : 512;
+constexpr uint32_t kGroupBytes = 16384;    // LDS for the groups' maxima, at most
 constexpr float kLowest = -3.402823466e38f;
 constexpr float kFarBelow = -1e30f;        // stands for -inf where it is multiplied by a zero probability
 constexpr float kLn2 = 0.69314718055994531f;
+constexpr float kReach = 1048576.0f;       // largest reference whose rounding is harmless
 
 // Order of floats as unsigned integers; both zeros are one value.
 __device__ __forceinline__ uint32_t Ordered(float x)
@@ -45,551 +53,800 @@ __device__ __forceinline__ uint64_t Key(uint32_t ordered, uint32_t index)
     return (static_cast<uint64_t>(ordered) << 32) | (0xFFFFFFFFu - index);
 }
 
+// Sums of a set of elements relative to a reference: kSafe: the largest logit itself, otherwise c * that.
 struct Stats {
     float m, s, t;
 };
 
-__device__ __forceinline__ void Rescale(Stats& a, float m, float exp2Scale)
+template <bool kSafe>
+__device__ __forceinline__ void Rescale(Stats& a, float m, float c)
 {
-    const float d = fmaxf((a.m - m) * exp2Scale, kFarBelow);
-    const float c = Exp2(d);
-    a.t = c * (a.t + a.s * d);
-    a.s = a.s * c;
+    const float d = kSafe ? fmaxf((a.m - m) * c, kFarBelow) : a.m - m;
+    const float f = Exp2(d);
+    a.t = f * __builtin_fmaf(a.s, d, a.t);
+    a.s = a.s * f;
     a.m = m;
 }
 
-// The same numbers for the union; both sides end up on the larger maximum.
-__device__ __forceinline__ Stats Join(Stats a, Stats b, float exp2Scale)
-{
-    const float m = fmaxf(a.m, b.m);
-    Rescale(a, m, exp2Scale);
-    Rescale(b, m, exp2Scale);
-    return Stats{m, a.s + b.s, a.t + b.t};
-}
-
-__device__ __forceinline__ Stats WaveJoin(Stats a, float exp2Scale)
+// The same for a wavefront's sets together.
+template <bool kSafe>
+__device__ __forceinline__ Stats WaveJoin(Stats a, float c)
 {
     Stats r;
-    r.m = WaveMax(a.m);
-    Rescale(a, r.m, exp2Scale);
+    r.m = LaneMax(a.m);
+    Rescale<kSafe>(a, r.m, c);
     r.s = WaveSum(a.s);
     r.t = WaveSum(a.t);
     return r;
 }
 
-template <uint32_t N>
-__device__ __forceinline__ void Accumulate(Stats& a, const float* x, float exp2Scale)
+template <bool kSafe>
+__device__ __forceinline__ Stats NoElements()
+{
+    return Stats{kSafe ? kLowest : -kReach, 0.0f, 0.0f};
+}
+
+// N more elements, of which the largest is returned; `largest` is the lane's largest logit so far.
+template <bool kSafe, uint32_t N>
+__device__ __forceinline__ float Accumulate(Stats& a, float& largest, const float* x, float c)
 {
     float most = x[0];
     for (uint32_t i = 1; i < N; ++i) {
         most = fmaxf(most, x[i]);
     }
-    if (most > a.m) {
-        Rescale(a, most, exp2Scale);
+    if (most > largest) {
+        largest = most;
+        Rescale<kSafe>(a, fmaxf(kSafe ? most : most * c, a.m), c);
     }
     for (uint32_t i = 0; i < N; ++i) {
-        const float y = (x[i] - a.m) * exp2Scale;
+        const float y = kSafe ? (x[i] - a.m) * c : __builtin_fmaf(x[i], c, -a.m);
         const float e = Exp2(y);
         a.s += e;
         a.t = __builtin_fmaf(fmaxf(y, kFarBelow), e, a.t);
     }
+    return most;
 }
 
-// The part of one shard's row that this workgroup reads: vectors [first, last) of which those below `full` are whole.
+// The vectors [first, last) of one part's row that this workgroup reads.  Those below `full` are whole; a shorter end of the
+// row is vector `full`, read as the last whole vector's worth of the row with the places before its elements masked.
 template <typename T>
-struct Range {
-    const typename T::Raw* row;
+struct Part {
+    typedef typename T::Raw Raw;
+    static constexpr uint32_t P = kPer16<T>;
+    static constexpr uint32_t kNone = sizeof(Raw) == 4 ? 0xFF800000u : T::kHalf ? 0xFC00FC00u : 0xFF80FF80u;   // -inf
+    const Raw* row;
     uint32_t count;
     uint32_t full;
     uint32_t first;
     uint32_t last;
 
-    __device__ __forceinline__ Range(const LogProbsArgs& a, uint32_t shard, uint64_t r, uint32_t split)
+    // `begin` is the number of vectors of the parts before it; the workgroup has the vectors [from, to) of them all.
+    __device__ __forceinline__ Part(const LogProbsArgs& a, uint32_t shard, uint64_t r, uint32_t begin, uint32_t from, uint32_t to)
     {
-        row = static_cast<const typename T::Raw*>(a.logits[shard]) + r * a.rowStride[shard];
+        row = static_cast<const Raw*>(a.logits[shard]) + r * a.rowStride[shard];
         count = a.count[shard];
-        full = count / kPer16<T>;
-        const uint32_t vectors = (count + kPer16<T> - 1) / kPer16<T>;
-        first = static_cast<uint32_t>(static_cast<uint64_t>(vectors) * split / a.nSplit);
-        last = static_cast<uint32_t>(static_cast<uint64_t>(vectors) * (split + 1) / a.nSplit);
-    }
-    // Elements of vector v; the places behind the end of the row get -inf.
-    __device__ __forceinline__ void Get(uint32_t v, float* x) const
-    {
-        if (v < full) {
-            Unpack16<T>(Load16(row + static_cast<uint64_t>(v) * kPer16<T>), x);
-        } else {
-            for (uint32_t i = 0; i < kPer16<T>; ++i) {
-                const uint32_t at = v * kPer16<T> + i;
-                x[i] = at < count ? Widen<T>(LoadOne(row + at)) : -__builtin_inff();
-            }
+        full = count / P;
+        const uint32_t end = begin + Vectors();
+        first = (from > begin ? from : begin) - begin;
+        last = (to < end ? to : end) - begin;
+        if (to <= begin || from >= end) {
+            first = last = 0;
         }
     }
+    __device__ __forceinline__ Part(const Raw* data, uint32_t n, uint32_t f, uint32_t l)
+        : row(data), count(n), full(n / P), first(f), last(l)
+    {
+    }
+    __device__ __forceinline__ uint32_t Vectors() const { return (count + P - 1) / P; }
+    // Places of vector v that hold an element of it, as bits.
     __device__ __forceinline__ uint32_t Valid(uint32_t v) const
     {
-        return v < full ? kPer16<T> : count - v * kPer16<T>;
+        const uint32_t all = (1u << P) - 1u, rest = count % P;
+        return v < full ? all : count >= P ? all & ~(all >> rest) : (1u << rest) - 1u;
+    }
+    // Index in the part's row of the first place of vector v.
+    __device__ __forceinline__ uint32_t Base(uint32_t v) const { return v < full ? v * P : count >= P ? count - P : 0u; }
+    __device__ __forceinline__ U32x4 Load(uint32_t v) const
+    {
+        if (v < full) {
+            return LoadOnce16(row + static_cast<uint64_t>(v) * P);
+        }
+        U32x4 raw = {kNone, kNone, kNone, kNone};
+        const uint32_t valid = Valid(v);
+        if (count >= P) {
+            raw = LoadOnce16(row + (count - P));
+        } else {
+            for (uint32_t i = 0; i < P; ++i) {
+                if (i < count) {
+                    Put(raw, i, LoadOne(row + i));
+                }
+            }
+        }
+        for (uint32_t i = 0; i < P; ++i) {
+            if (!((valid >> i) & 1u)) {
+                Put(raw, i, static_cast<Raw>(kNone));
+            }
+        }
+        return raw;
+    }
+    static __device__ __forceinline__ void Put(U32x4& raw, uint32_t i, Raw e)
+    {
+        if constexpr (sizeof(Raw) == 4) {
+            raw[i] = e;
+        } else {
+            const uint32_t keep = raw[i / 2] & (0xFFFFu << (16 * ((i + 1) % 2)));
+            raw[i / 2] = keep | (static_cast<uint32_t>(e) << (16 * (i % 2)));
+        }
     }
 };
 
-// Descending bitonic sort of one value per lane.
-__device__ __forceinline__ uint32_t WaveSort(uint32_t v, uint32_t lane)
+// Hands out the workgroup's vectors, kUnroll per lane at a time.
+template <typename T, uint32_t kThreads>
+struct Reader {
+    const LogProbsArgs& a;
+    uint64_t row;
+    uint32_t from, to;       // flat vectors of this workgroup
+    uint32_t shard = 0;
+    uint32_t begin = 0;      // vectors of the parts before `shard`
+    uint32_t next = 0;       // next vector of the current part
+    Part<T> part;
+    bool any = false;        // the lane has had an element
+
+    __device__ __forceinline__ Reader(const LogProbsArgs& args, uint64_t r, uint32_t f, uint32_t t)
+        : a(args), row(r), from(f), to(t), part(args, 0, r, 0, f, t)
+    {
+        next = part.first;
+    }
+    __device__ __forceinline__ bool Fetch(U32x4* raw)
+    {
+        while (next >= part.last) {
+            begin += part.Vectors();
+            if (++shard >= a.nShards || begin >= to) {
+                return false;
+            }
+            part = Part<T>(a, shard, row, begin, from, to);
+            next = part.first;
+        }
+        const uint32_t v = next + threadIdx.x;
+        if (next + kThreads * kUnroll <= (part.last < part.full ? part.last : part.full)) {
+            for (uint32_t u = 0; u < kUnroll; ++u) {
+                raw[u] = LoadOnce16(part.row + static_cast<uint64_t>(v + u * kThreads) * Part<T>::P);
+            }
+            any = true;
+        } else {
+            for (uint32_t u = 0; u < kUnroll; ++u) {
+                raw[u] = U32x4{Part<T>::kNone, Part<T>::kNone, Part<T>::kNone, Part<T>::kNone};
+                if (v + u * kThreads < part.last) {
+                    raw[u] = part.Load(v + u * kThreads);
+                    any = true;
+                }
+            }
+        }
+        next += kThreads * kUnroll;
+        return true;
+    }
+};
+
+// How many of the n keys are larger; eight at a time, so that their reads do not wait for each other.
+__device__ __forceinline__ uint32_t RankOf(uint64_t key, const uint64_t* keys, uint32_t n)
 {
-    for (uint32_t size = 2; size <= kWave; size <<= 1) {
-        for (uint32_t d = size >> 1; d > 0; d >>= 1) {
-            const uint32_t o = __shfl_xor(v, d);
-            const bool keepMax = ((lane & d) == 0) == ((lane & size) == 0);
-            v = keepMax ? (v > o ? v : o) : (v < o ? v : o);
+    uint32_t rank = 0, o = 0;
+    for (; o + 8 <= n; o += 8) {
+        uint64_t k[8];
+        for (uint32_t i = 0; i < 8; ++i) {
+            k[i] = keys[o + i];
+        }
+        for (uint32_t i = 0; i < 8; ++i) {
+            rank += k[i] > key ? 1 : 0;
         }
     }
-    return v;
-}
-
-// Sorts a bitonic sequence of 32 in each half of the wavefront, descending.
-__device__ __forceinline__ uint32_t HalfMerge(uint32_t v, uint32_t lane)
-{
-    for (uint32_t d = 16; d > 0; d >>= 1) {
-        const uint32_t o = __shfl_xor(v, d);
-        v = (lane & d) == 0 ? (v > o ? v : o) : (v < o ? v : o);
+    for (; o < n; ++o) {
+        rank += keys[o] > key ? 1 : 0;
     }
-    return v;
+    return rank;
 }
 
+constexpr uint32_t kBins = 256;
+template <uint32_t kThreads>
 struct TopSpace {
-    uint32_t sorted[kWaves][32];
-    uint32_t lanes[kThreads];
-    uint64_t candidate[kCandidates];
-    uint32_t nLanes;
+    uint32_t bin[kBins];
+    uint32_t group[kCandidates<kThreads>];       // groups that reach the bound: slot << 16 | lane
+    uint64_t candidate[kCandidates<kThreads>];
+    uint64_t top[kMaxTop];
+    uint32_t waveCount[kThreads / kWave];
+    uint32_t nGroups;
     uint32_t nCandidates;
-    uint32_t bound;
-    uint32_t total;
-    uint32_t waveCount[kWaves];
 };
 
 // Sum over the workgroup; every thread gets it.
-__device__ __forceinline__ uint32_t BlockCount(uint32_t v, TopSpace& sh, uint32_t tid)
+template <uint32_t kThreads>
+__device__ __forceinline__ uint32_t BlockCount(uint32_t v, TopSpace<kThreads>& sh, uint32_t tid)
 {
-    for (int d = 32; d > 0; d >>= 1) {
-        v += __shfl_xor(v, d);
-    }
+    v = WaveSum(v);
     __syncthreads();
     if ((tid & (kWave - 1)) == 0) {
         sh.waveCount[tid / kWave] = v;
     }
     __syncthreads();
     uint32_t sum = 0;
-    for (uint32_t w = 0; w < kWaves; ++w) {
+    for (uint32_t w = 0; w < kThreads / kWave; ++w) {
         sum += sh.waveCount[w];
     }
     return sum;
 }
 
-// Elements of the workgroup's part of the row whose order is at least (or, above = true, above) `bound`.
-template <typename T>
-__device__ __forceinline__ uint32_t CountFrom(const LogProbsArgs& a, uint64_t row, uint32_t split, uint32_t bound, bool above, TopSpace& sh,
-                              uint32_t tid)
+// Elements of the workgroup's part of the row whose order is at least `bound`.
+template <typename T, uint32_t kThreads>
+__device__ __forceinline__ uint32_t CountFrom(const LogProbsArgs& a, uint64_t row, uint32_t from, uint32_t to, uint32_t bound,
+                                              TopSpace<kThreads>& sh, uint32_t tid)
 {
-    uint32_t n = 0;
+    uint32_t n = 0, begin = 0;
     for (uint32_t shard = 0; shard < a.nShards; ++shard) {
-        const Range<T> r(a, shard, row, split);
-        for (uint32_t v = r.first + tid; v < r.last; v += kThreads) {
+        const Part<T> part(a, shard, row, begin, from, to);
+        for (uint32_t v = part.first + tid; v < part.last; v += kThreads) {
             float x[kPer16<T>];
-            r.Get(v, x);
-            const uint32_t valid = r.Valid(v);
+            Unpack16<T>(part.Load(v), x);
+            const uint32_t valid = part.Valid(v);
             for (uint32_t i = 0; i < kPer16<T>; ++i) {
-                const uint32_t o = Ordered(x[i]);
-                n += (i < valid && (above ? o > bound : o >= bound)) ? 1 : 0;
+                n += ((valid >> i) & 1u) != 0 && Ordered(x[i]) >= bound ? 1 : 0;
             }
         }
+        begin += part.Vectors();
     }
     return BlockCount(n, sh, tid);
 }
 
-// The exact search, for rows with more elements at the bound than the list holds: the topCount-th largest logit by
-// bisection, then everything above it and, in ascending order, as many equal to it as are still wanted.  A dozen or more
-// passes over the (cached) row in general, two where the bound itself is the largest logit, as in a row of equal ones.
-template <typename T>
-__device__ __forceinline__ void SearchTop(const LogProbsArgs& a, uint64_t row, uint32_t split, uint32_t most, TopSpace& sh,
-                                       uint32_t tid)
+// Appends the first `want` elements of the workgroup's part of the row whose order is `value`, in ascending order.
+template <typename T, uint32_t kThreads>
+__device__ __forceinline__ void FirstEqual(const LogProbsArgs& a, uint64_t row, uint32_t from, uint32_t to, uint32_t value,
+                                           uint32_t want, TopSpace<kThreads>& sh, uint32_t tid)
 {
-    uint32_t low = sh.bound;       // at least topCount elements reach it
-    uint32_t high = most;          // nothing lies above it
-    uint32_t above = CountFrom<T>(a, row, split, low, true, sh, tid);
-    if (above >= a.topCount) {
-        while (low < high) {       // the largest value that topCount elements reach
+    uint32_t start = 0, begin = 0;
+    for (uint32_t shard = 0; shard < a.nShards && want != 0; ++shard) {
+        const Part<T> part(a, shard, row, begin, from, to);
+        for (uint32_t v0 = part.first; v0 < part.last && want != 0; v0 += kThreads) {
+            const uint32_t v = v0 + tid;
+            uint32_t equal = 0;     // bit i: place i equals `value`
+            if (v < part.last) {
+                float x[kPer16<T>];
+                Unpack16<T>(part.Load(v), x);
+                for (uint32_t i = 0; i < kPer16<T>; ++i) {
+                    equal |= Ordered(x[i]) == value ? 1u << i : 0u;
+                }
+                equal &= part.Valid(v);
+            }
+            // position of the lane's first one among those of all lanes
+            const uint32_t mine = __popc(equal), upTo = WaveScan(mine);
+            __syncthreads();
+            if ((tid & (kWave - 1)) == kWave - 1) {
+                sh.waveCount[tid / kWave] = upTo;
+            }
+            __syncthreads();
+            uint32_t before = upTo - mine, total = 0;
+            for (uint32_t w = 0; w < kThreads / kWave; ++w) {
+                before += w < tid / kWave ? sh.waveCount[w] : 0;
+                total += sh.waveCount[w];
+            }
+            for (uint32_t i = 0; i < kPer16<T>; ++i) {
+                if ((equal >> i) & 1u) {
+                    if (before < want) {
+                        sh.candidate[atomicAdd(&sh.nCandidates, 1u)] = Key(value, start + part.Base(v) + i);
+                    }
+                    ++before;
+                }
+            }
+            want -= total < want ? total : want;
+        }
+        start += part.count;
+        begin += part.Vectors();
+    }
+    __syncthreads();
+}
+
+// The search that needs no list, for rows in which a few lanes hold more large elements than the list takes: the
+// topCount-th largest logit by bisection, then everything above it.  Returns it; some thirty passes over the row.
+template <typename T, uint32_t kThreads>
+__device__ __forceinline__ uint32_t SearchTop(const LogProbsArgs& a, uint64_t row, uint32_t from, uint32_t to, uint32_t low,
+                                              uint32_t high, TopSpace<kThreads>& sh, uint32_t tid)
+{
+    // at least topCount elements reach `low`, none lies above `high`
+    while (low < high) {       // the largest value that topCount elements reach
+        const uint32_t mid = low + (high - low + 1) / 2;
+        if (CountFrom<T>(a, row, from, to, mid, sh, tid) >= a.topCount) {
+            low = mid;
+        } else {
+            high = mid - 1;
+        }
+    }
+    __syncthreads();
+    if (tid == 0) {
+        sh.nCandidates = 0;
+    }
+    __syncthreads();
+    uint32_t start = 0, begin = 0;
+    for (uint32_t shard = 0; shard < a.nShards; ++shard) {
+        const Part<T> part(a, shard, row, begin, from, to);
+        for (uint32_t v = part.first + tid; v < part.last; v += kThreads) {
+            float x[kPer16<T>];
+            Unpack16<T>(part.Load(v), x);
+            const uint32_t valid = part.Valid(v);
+            for (uint32_t i = 0; i < kPer16<T>; ++i) {
+                const uint32_t o = Ordered(x[i]);
+                if (((valid >> i) & 1u) != 0 && o > low) {
+                    sh.candidate[atomicAdd(&sh.nCandidates, 1u)] = Key(o, start + part.Base(v) + i);
+                }
+            }
+        }
+        start += part.count;
+        begin += part.Vectors();
+    }
+    __syncthreads();
+    return low;
+}
+
+// A value that `want` lanes reach, or 0 if there are fewer lanes with an element: the lower edge of the first bin of the
+// histogram, counted from the largest value on, up to which `want` lane maxima fall; `reaching` counts them.  Bins are
+// 2^shift orders wide, first as fine as bfloat16, and wider where the first 255 do not reach far enough.  Every wavefront
+// reads the histogram for itself.
+template <uint32_t kThreads>
+__device__ __forceinline__ uint32_t TopBound(uint32_t laneMost, uint32_t largest, uint32_t want, uint32_t& reaching,
+                                             TopSpace<kThreads>& sh, uint32_t tid)
+{
+    const uint32_t lane = tid & (kWave - 1);
+    for (uint32_t shift = 16;; shift += 4) {
+        const uint32_t far = (largest - laneMost) >> shift;
+        if (laneMost != 0) {
+            atomicAdd(&sh.bin[far < kBins - 1 ? far : kBins - 1], 1u);
+        }
+        __syncthreads();
+        uint32_t n[4], sum = 0;
+        for (uint32_t i = 0; i < 4; ++i) {
+            n[i] = sh.bin[4 * lane + i];
+            sum += n[i];
+        }
+        const uint32_t upTo = WaveScan(sum);
+        const uint64_t reached = __ballot(upTo >= want);
+        if (reached == 0) {
+            reaching = __builtin_amdgcn_readlane(upTo, kWave - 1);
+            return 0;
+        }
+        const uint32_t at = __ffsll(static_cast<unsigned long long>(reached)) - 1;
+        uint32_t bin = 4 * at;
+        reaching = __builtin_amdgcn_readlane(upTo - sum, at);
+        for (uint32_t i = 0; i < 4 && reaching < want; ++i) {
+            reaching += __builtin_amdgcn_readlane(n[i], at);
+            bin += reaching < want ? 1 : 0;
+        }
+        if (bin < kBins - 1 || shift >= 24) {
+            // the bin holds orders in (largest - ((bin + 1) << shift), largest - (bin << shift)]
+            const uint64_t depth = ((static_cast<uint64_t>(bin) + 1) << shift) - 1;
+            return depth < largest ? largest - static_cast<uint32_t>(depth) : 1u;
+        }
+        __syncthreads();
+        for (uint32_t i = tid; i < kBins; i += kThreads) {
+            sh.bin[i] = 0;
+        }
+        __syncthreads();
+    }
+}
+
+// Lists the groups of this lane that reach `bound`, reads them again and lists their elements that do.  False if there are
+// more of either than a list takes.
+template <typename T, uint32_t kThreads>
+__device__ __forceinline__ bool ListElements(const LogProbsArgs& a, uint64_t row, uint32_t from, uint32_t to, uint32_t laneMost,
+                                             uint32_t bound, uint32_t nSlots, const uint16_t* groupMost, TopSpace<kThreads>& sh,
+                                             uint32_t tid)
+{
+    constexpr uint32_t P = kPer16<T>;
+    if (laneMost != 0 && laneMost >= bound) {
+        for (uint32_t slot = 0; slot < nSlots; ++slot) {
+            if (groupMost[slot * kThreads + tid] >= bound >> 16) {
+                const uint32_t at = atomicAdd(&sh.nGroups, 1u);
+                if (at < kCandidates<kThreads>) {
+                    sh.group[at] = slot << 16 | tid;
+                }
+            }
+        }
+    }
+    __syncthreads();
+    // A slot is 2^slotShift fetches of kUnroll vectors of the lane; one thread per vector.
+    const uint32_t nGroups = sh.nGroups;
+    if (nGroups > kCandidates<kThreads>) {
+        return false;
+    }
+    const float least = bound <= Ordered(-__builtin_inff()) ? -__builtin_inff() : FromOrdered(bound);
+    const uint32_t fetches = 1u << a.slotShift;
+    for (uint32_t item = tid; item < nGroups * (fetches * kUnroll); item += kThreads) {
+        const uint32_t group = sh.group[item / (fetches * kUnroll)];
+        const uint32_t fetch = (group >> 16) * fetches + item / kUnroll % fetches;
+        uint32_t begin = 0, start = 0, before = 0;
+        uint32_t v = 0, last = 0, count = 0, index = 0;
+        const typename T::Raw* data = nullptr;
+        for (uint32_t shard = 0; shard < a.nShards && begin < to; ++shard) {
+            const Part<T> part(a, shard, row, begin, from, to);
+            const uint32_t per = (part.last - part.first + kThreads * kUnroll - 1) / (kThreads * kUnroll);
+            if (fetch - before < per) {       // (below `before` the difference wraps and is not)
+                data = part.row;
+                v = part.first + ((fetch - before) * kUnroll + item % kUnroll) * kThreads + (group & 0xFFFFu);
+                last = part.last;
+                count = part.count;
+                index = start;
+            }
+            before += per;
+            start += part.count;
+            begin += part.Vectors();
+        }
+        if (v < last) {
+            const Part<T> part(data, count, 0, last);
+            float x[P];
+            Unpack16<T>(part.Load(v), x);
+            const uint32_t valid = part.Valid(v);
+            index += part.Base(v);
+            for (uint32_t e = 0; e < P; ++e) {
+                if (x[e] >= least && ((valid >> e) & 1u) != 0) {
+                    const uint32_t c = atomicAdd(&sh.nCandidates, 1u);
+                    if (c < kCandidates<kThreads>) {
+                        sh.candidate[c] = Key(Ordered(x[e]), index + e);
+                    }
+                }
+            }
+        }
+    }
+    __syncthreads();
+    return sh.nCandidates <= kCandidates<kThreads>;
+}
+
+// Leaves the topCount largest keys of the workgroup's part of the row in sh.top, descending, 0 where there is none.
+// laneMost: order of the lane's largest logit, 0 if it had no element; largest: of the workgroup's.  sh.bin, sh.top and the
+// counters are zero.
+template <typename T, uint32_t kThreads>
+__device__ __forceinline__ void GatherTop(const LogProbsArgs& a, uint64_t row, uint32_t from, uint32_t to, uint32_t laneMost,
+                                          uint32_t largest, uint32_t nSlots, const uint16_t* groupMost, TopSpace<kThreads>& sh,
+                                          uint32_t tid)
+{
+    uint32_t reaching;
+    const uint32_t bound = TopBound<kThreads>(laneMost, largest, a.topCount, reaching, sh, tid);
+    // (with fewer lanes than topCount, or a list that a few lanes more than fill, there is nothing to be gained from trying)
+    const bool few = reaching <= kCandidates<kThreads> / 4 &&
+                     ListElements<T, kThreads>(a, row, from, to, laneMost, bound, nSlots, groupMost, sh, tid);
+    if (!few) {
+        uint32_t low = bound, high = largest;      // the exact topCount-th lane maximum
+        while (low < high && reaching >= a.topCount) {
             const uint32_t mid = low + (high - low + 1) / 2;
-            if (CountFrom<T>(a, row, split, mid, false, sh, tid) >= a.topCount) {
+            if (BlockCount<kThreads>(laneMost >= mid ? 1 : 0, sh, tid) >= a.topCount) {
                 low = mid;
             } else {
                 high = mid - 1;
             }
         }
-        above = CountFrom<T>(a, row, split, low, true, sh, tid);
-    }
-    uint32_t want = a.topCount - above;    // of those equal to `low`
-    __syncthreads();
-    if (tid == 0) {
-        sh.nCandidates = 0;
-    }
-    __syncthreads();
-    uint32_t start = 0;
-    for (uint32_t shard = 0; shard < a.nShards; ++shard) {
-        const Range<T> r(a, shard, row, split);
-        for (uint32_t v0 = r.first; v0 < r.last; v0 += kThreads) {
-            const uint32_t v = v0 + tid;
-            uint32_t equal = 0;     // bit i: element i equals `low`
-            if (v < r.last) {
-                float x[kPer16<T>];
-                r.Get(v, x);
-                const uint32_t valid = r.Valid(v);
-                for (uint32_t i = 0; i < kPer16<T>; ++i) {
-                    const uint32_t o = Ordered(x[i]);
-                    if (i < valid && o > low) {
-                        sh.candidate[atomicAdd(&sh.nCandidates, 1u)] = Key(o, start + v * kPer16<T> + i);
-                    }
-                    equal |= (i < valid && o == low) ? 1u << i : 0u;
-                }
-            }
-            if (want != 0) {
-                // position of the lane's first equal element among those of all lanes
-                const uint32_t mine = __popc(equal);
-                uint32_t before = mine;
-                for (uint32_t d = 1; d < kWave; d <<= 1) {
-                    const uint32_t o = __shfl_up(before, d);
-                    before += (tid & (kWave - 1)) >= d ? o : 0;
-                }
-                __syncthreads();
-                if ((tid & (kWave - 1)) == kWave - 1) {
-                    sh.waveCount[tid / kWave] = before;
-                }
-                __syncthreads();
-                uint32_t total = 0;
-                before -= mine;
-                for (uint32_t w = 0; w < kWaves; ++w) {
-                    before += w < tid / kWave ? sh.waveCount[w] : 0;
-                    total += sh.waveCount[w];
-                }
-                for (uint32_t i = 0; i < kPer16<T>; ++i) {
-                    if ((equal >> i) & 1u) {
-                        if (before < want) {
-                            sh.candidate[atomicAdd(&sh.nCandidates, 1u)] = Key(low, start + v * kPer16<T> + i);
-                        }
-                        ++before;
-                    }
-                }
-                want -= total < want ? total : want;
-            }
+        __syncthreads();
+        if (tid == 0) {
+            sh.nGroups = 0;
+            sh.nCandidates = 0;
         }
-        start += r.count;
-    }
-    __syncthreads();
-}
-
-// Leaves at least the topCount largest keys of the workgroup's part of the row (all keys if it is shorter) in
-// sh.candidate, at most kCandidates.  laneMost: order of the lane's largest logit, 0 if it had no element.
-template <typename T>
-__device__ __forceinline__ void GatherTop(const LogProbsArgs& a, uint64_t row, uint32_t split, uint32_t laneMost, TopSpace& sh, uint32_t tid)
-{
-    const uint32_t lane = tid & (kWave - 1);
-    const uint32_t sorted = WaveSort(laneMost, lane);
-    if (lane < 32) {
-        sh.sorted[tid / kWave][lane] = sorted;
-    }
-    if (tid == 0) {
-        sh.nLanes = 0;
-        sh.nCandidates = 0;
-    }
-    __syncthreads();
-    if (tid < kWave) {
-        // lanes 0..31: the 32 largest of wavefronts 0 and 1, lanes 32..63: of 2 and 3; then of both
-        const uint32_t i = lane & 31u, pair = (lane >> 5) * 2;
-        const uint32_t x = sh.sorted[pair][i], y = sh.sorted[pair + 1][31 - i];
-        uint32_t v = HalfMerge(x > y ? x : y, lane);
-        const uint32_t o = __shfl(v, 63 - lane);
-        v = HalfMerge(v > o ? v : o, lane);
-        if (lane == 0) {
-            sh.total = v;          // the largest
+        __syncthreads();
+        if (!ListElements<T, kThreads>(a, row, from, to, laneMost, low + 1, nSlots, groupMost, sh, tid)) {
+            low = SearchTop<T, kThreads>(a, row, from, to, low, largest, sh, tid);
         }
-        if (lane == a.topCount - 1) {
-            sh.bound = v;
+        const uint32_t n = sh.nCandidates;
+        if (n < a.topCount) {
+            FirstEqual<T, kThreads>(a, row, from, to, low, a.topCount - n, sh, tid);
+        }
+    }
+    const uint32_t n = sh.nCandidates;
+    for (uint32_t c = tid; c < n; c += kThreads) {
+        const uint64_t key = sh.candidate[c];
+        const uint32_t rank = RankOf(key, sh.candidate, n);
+        if (rank < a.topCount) {
+            sh.top[rank] = key;
         }
     }
     __syncthreads();
-    const uint32_t bound = sh.bound;
-    if (laneMost != 0 && laneMost >= bound) {
-        sh.lanes[atomicAdd(&sh.nLanes, 1u)] = tid;
-    }
-    __syncthreads();
-    const uint32_t nLanes = sh.nLanes;
-    uint32_t start = 0;
-    for (uint32_t shard = 0; shard < a.nShards; ++shard) {
-        const Range<T> r(a, shard, row, split);
-        const uint32_t perLane = (r.last - r.first + kThreads - 1) / kThreads;
-        for (uint32_t item = tid; item < nLanes * perLane; item += kThreads) {
-            const uint32_t j = item / nLanes;
-            const uint32_t v = r.first + j * kThreads + sh.lanes[item - j * nLanes];
-            if (v < r.last) {
-                float x[kPer16<T>];
-                r.Get(v, x);
-                const uint32_t valid = r.Valid(v);
-                for (uint32_t i = 0; i < kPer16<T>; ++i) {
-                    const uint32_t o = Ordered(x[i]);
-                    if (i < valid && o >= bound) {
-                        const uint32_t at = atomicAdd(&sh.nCandidates, 1u);
-                        if (at < kCandidates) {
-                            sh.candidate[at] = Key(o, start + v * kPer16<T> + i);
-                        }
-                    }
-                }
-            }
-        }
-        start += r.count;
-    }
-    __syncthreads();
-    if (sh.nCandidates > kCandidates) {
-        SearchTop<T>(a, row, split, sh.total, sh, tid);
-    }
 }
 
 // What is written for a row once its numbers are known.
 struct RowResult {
-    float m, logSum, lse, entropy;
+    float m, log2Sum, lse, entropy;
+    bool safe;      // how m is meant, see Stats
     bool none;      // -inf alone
     bool bad;       // a NaN or +inf
 };
 
-__device__ __forceinline__ RowResult Finish(Stats a, float scale)
+__device__ __forceinline__ RowResult Finish(Stats a, bool safe, const LogProbsArgs& k)
 {
     RowResult r;
     r.m = a.m;
+    r.safe = safe;
     r.none = a.s == 0.0f;
     r.bad = a.s != a.s;
-    r.logSum = logf(a.s);
-    r.lse = r.none ? -__builtin_inff() : a.m * scale + r.logSum;
-    r.entropy = r.none ? 0.0f : r.logSum - kLn2 * (a.t / a.s);
+    r.log2Sum = log2f(a.s);
+    r.lse = r.none ? -__builtin_inff() : safe ? __builtin_fmaf(a.m, k.scale, r.log2Sum * kLn2) : (a.m + r.log2Sum) * kLn2;
+    r.entropy = r.none ? 0.0f : kLn2 * (r.log2Sum - a.t / a.s);
     return r;
 }
 
-__device__ __forceinline__ float LogProbOf(const RowResult& r, float x, float scale)
+__device__ __forceinline__ float LogProbOf(const RowResult& r, float x, const LogProbsArgs& k)
 {
-    return r.none ? -__builtin_inff() : (x - r.m) * scale - r.logSum;
+    const float y = r.safe ? (x - r.m) * k.exp2Scale : __builtin_fmaf(x, k.exp2Scale, -r.m);
+    // (far below the others the logit itself decides, and c x may be beyond a float where scale x is not)
+    return r.none ? -__builtin_inff() : y < -kReach ? __builtin_fmaf(x, k.scale, -r.lse) : kLn2 * (y - r.log2Sum);
 }
 
+// The given token of a row and its logit, fetched before the reductions that the result waits for.
+struct Token {
+    int64_t id;
+    float logit;
+};
 template <typename T>
-__device__ __forceinline__ void WriteRow(const LogProbsArgs& a, uint64_t row, const RowResult& r)
+__device__ __forceinline__ float TokenLogit(const LogProbsArgs& a, uint64_t row, int64_t token)
 {
-    float logProb = 0.0f;
-    if (a.tokens != nullptr) {
-        const int64_t token = a.wideTokens ? LoadOne(static_cast<const int64_t*>(a.tokens) + row)
-                                           : LoadOne(static_cast<const int32_t*>(a.tokens) + row);
-        if (token >= a.vocab) {
-            logProb = __builtin_nanf("");
-        } else if (token >= 0) {
-            uint32_t at = static_cast<uint32_t>(token);
-            uint32_t shard = 0;
-            while (at >= a.count[shard]) {
-                at -= a.count[shard];
-                ++shard;
-            }
-            const typename T::Raw* p = static_cast<const typename T::Raw*>(a.logits[shard]) + row * a.rowStride[shard] + at;
-            logProb = LogProbOf(r, Widen<T>(LoadOne(p)), a.scale);
+    if (token < 0 || token >= a.vocab) {
+        return 0.0f;
+    }
+    uint32_t at = static_cast<uint32_t>(token);
+    uint32_t shard = 0;
+    while (at >= a.count[shard]) {
+        at -= a.count[shard];
+        ++shard;
+    }
+    return Widen<T>(LoadOne(static_cast<const typename T::Raw*>(a.logits[shard]) + row * a.rowStride[shard] + at));
+}
+__device__ __forceinline__ int64_t TokenId(const LogProbsArgs& a, uint64_t row)
+{
+    return a.tokens == nullptr ? -1
+           : a.wideTokens      ? LoadOne(static_cast<const int64_t*>(a.tokens) + row)
+                               : LoadOne(static_cast<const int32_t*>(a.tokens) + row);
+}
+
+// Every rank's outputs, a wavefront per rank.
+template <uint32_t kThreads>
+__device__ __forceinline__ void WriteRow(const LogProbsArgs& a, uint64_t row, const RowResult& r, Token token, const uint64_t* top)
+{
+    const uint32_t lane = threadIdx.x & (kWave - 1);
+    float value = 0.0f;
+    int64_t id = -1;
+    if (lane < a.topCount) {
+        value = __builtin_nanf("");
+        if (!r.bad) {
+            const uint64_t key = top[lane];
+            value = LogProbOf(r, FromOrdered(static_cast<uint32_t>(key >> 32)), a);
+            id = static_cast<int64_t>(0xFFFFFFFFu - static_cast<uint32_t>(key));
         }
     }
-    for (uint32_t o = 0; o < a.nOut; ++o) {
-        if (a.out[o].logProbs != nullptr) {
-            StoreOne(a.out[o].logProbs + row, logProb);
+    const float logProb = token.id >= a.vocab ? __builtin_nanf("") : token.id >= 0 ? LogProbOf(r, token.logit, a) : 0.0f;
+    for (uint32_t o = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave); o < a.nOut; o += kThreads / kWave) {
+        const LogProbsArgs::Out& out = a.out[o];
+        if (lane == 0) {
+            if (out.logProbs != nullptr) {
+                StoreOne(out.logProbs + row, logProb);
+            }
+            if (out.logSumExp != nullptr) {
+                StoreOne(out.logSumExp + row, r.lse);
+            }
+            if (out.entropy != nullptr) {
+                StoreOne(out.entropy + row, r.entropy);
+            }
         }
-        if (a.out[o].logSumExp != nullptr) {
-            StoreOne(a.out[o].logSumExp + row, r.lse);
-        }
-        if (a.out[o].entropy != nullptr) {
-            StoreOne(a.out[o].entropy + row, r.entropy);
+        if (lane < a.topCount) {
+            const uint64_t at = row * a.topCount + lane;
+            if (out.topValues != nullptr) {
+                StoreOne(out.topValues + at, value);
+            }
+            if (out.topIds != nullptr) {
+                if (a.wideTokens) {
+                    StoreOne(static_cast<int64_t*>(out.topIds) + at, id);
+                } else {
+                    StoreOne(static_cast<int32_t*>(out.topIds) + at, static_cast<int32_t>(id));
+                }
+            }
         }
     }
 }
 
-__device__ __forceinline__ void WriteTop(const LogProbsArgs& a, uint64_t row, const RowResult& r, uint32_t rank, uint64_t key)
+// One pass over the workgroup's part of the row, joined over the workgroup; `largest` is the lane's largest logit, and with
+// kTop groupMost[slot][lane] the order, cut to 16 bits, of the largest of 2^slotShift fetches.
+template <typename T, uint32_t kThreads, bool kTop, bool kSafe>
+__device__ __forceinline__ Stats Pass(const LogProbsArgs& a, uint64_t row, uint32_t from, uint32_t to, Stats* waveStats,
+                                      float* waveMost, float& largest, bool& any, uint16_t* groupMost, uint32_t& nSlots, Token& token)
 {
-    const float value = r.bad ? __builtin_nanf("") : LogProbOf(r, FromOrdered(static_cast<uint32_t>(key >> 32)), a.scale);
-    const int64_t id = r.bad ? -1 : static_cast<int64_t>(0xFFFFFFFFu - static_cast<uint32_t>(key));
-    const uint64_t at = row * a.topCount + rank;
-    for (uint32_t o = 0; o < a.nOut; ++o) {
-        if (a.out[o].topValues != nullptr) {
-            StoreOne(a.out[o].topValues + at, value);
+    constexpr uint32_t kWaves = kThreads / kWave;
+    const uint32_t lane = threadIdx.x & (kWave - 1);
+    Stats acc = NoElements<kSafe>();
+    largest = -__builtin_inff();
+    Reader<T, kThreads> reader(a, row, from, to);
+    U32x4 raw[kUnroll];
+    uint32_t fetch = 0, slotMost = 0;
+    while (reader.Fetch(raw)) {
+        float x[kUnroll * kPer16<T>];
+        for (uint32_t u = 0; u < kUnroll; ++u) {
+            Unpack16<T>(raw[u], x + u * kPer16<T>);
         }
-        if (a.out[o].topIds != nullptr) {
-            if (a.wideTokens) {
-                StoreOne(static_cast<int64_t*>(a.out[o].topIds) + at, id);
-            } else {
-                StoreOne(static_cast<int32_t*>(a.out[o].topIds) + at, static_cast<int32_t>(id));
-            }
+        if (!kSafe && fetch == 0) {
+            token.logit = TokenLogit<T>(a, row, token.id);      // on its way while the row is read
         }
+        const float most = Accumulate<kSafe, kUnroll * kPer16<T>>(acc, largest, x, a.exp2Scale);
+        if constexpr (kTop) {
+            const uint32_t order = Ordered(most) >> 16;
+            slotMost = (fetch & ((1u << a.slotShift) - 1u)) != 0 && slotMost > order ? slotMost : order;
+            groupMost[(fetch >> a.slotShift) * kThreads + threadIdx.x] = static_cast<uint16_t>(slotMost);
+        }
+        ++fetch;
     }
-}
-
-template <typename T, bool kTop>
-__global__ __launch_bounds__(kThreads) void LogProbsKernel(const LogProbsArgs a)
-{
-    constexpr uint32_t P = kPer16<T>;
-    __shared__ Stats waveStats[kWaves];
-    const uint32_t tid = threadIdx.x;
-    const uint32_t split = blockIdx.x % a.nSplit;
-    const uint64_t row = blockIdx.x / a.nSplit;
-    Stats acc = {kLowest, 0.0f, 0.0f};
-    bool any = false;
-    for (uint32_t shard = 0; shard < a.nShards; ++shard) {
-        const Range<T> r(a, shard, row, split);
-        const uint32_t whole = r.last < r.full ? r.last : r.full;
-        uint32_t v = r.first;
-        for (; v + kThreads * kUnroll <= whole; v += kThreads * kUnroll) {
-            U32x4 raw[kUnroll];
-            for (uint32_t u = 0; u < kUnroll; ++u) {
-                raw[u] = LoadOnce16(r.row + static_cast<uint64_t>(v + u * kThreads + tid) * P);
-            }
-            float x[kUnroll * P];
-            for (uint32_t u = 0; u < kUnroll; ++u) {
-                Unpack16<T>(raw[u], x + u * P);
-            }
-            Accumulate<kUnroll * P>(acc, x, a.exp2Scale);
-            any = true;
-        }
-        for (v += tid; v < r.last; v += kThreads) {
-            float x[P];
-            r.Get(v, x);
-            Accumulate<P>(acc, x, a.exp2Scale);
-            any = true;
-        }
-    }
-    const Stats wave = WaveJoin(acc, a.exp2Scale);
-    if ((tid & (kWave - 1)) == 0) {
-        waveStats[tid / kWave] = wave;
+    nSlots = (fetch + (1u << a.slotShift) - 1) >> a.slotShift;
+    any = reader.any;
+    const Stats wave = WaveJoin<kSafe>(acc, a.exp2Scale);
+    const float most = LaneMax(largest);
+    if (lane == 0) {
+        waveStats[threadIdx.x / kWave] = wave;
+        waveMost[threadIdx.x / kWave] = most;
     }
     __syncthreads();
-    Stats all = waveStats[0];
-    for (uint32_t w = 1; w < kWaves; ++w) {
-        all = Join(all, waveStats[w], a.exp2Scale);
+    Stats all = NoElements<kSafe>();
+    if (lane < kWaves) {
+        all = waveStats[lane];
     }
-    const RowResult result = Finish(all, a.scale);
-    if (tid == 0) {
-        if (a.nSplit == 1) {
-            WriteRow<T>(a, row, result);
-        } else {
-            float* p = a.stats + (row * a.nSplit + split) * 4;
-            StoreOne(p, all.m);
-            StoreOne(p + 1, all.s);
-            StoreOne(p + 2, all.t);
+    return WaveJoin<kSafe>(all, a.exp2Scale);
+}
+
+template <typename T, uint32_t kThreads, bool kTop>
+__global__ __launch_bounds__(kThreads, kThreads > 256 ? 4 : kTop ? 7 : 8) void LogProbsKernel(const LogProbsArgs a)
+{
+    constexpr uint32_t kWaves = kThreads / kWave;
+    __shared__ Stats waveStats[2][kWaves];
+    __shared__ float waveMost[kWaves];
+    __shared__ TopSpace<kTop ? kThreads : kWave> sh;
+    extern __shared__ uint16_t groupMost[];
+    const uint32_t tid = threadIdx.x, lane = tid & (kWave - 1);
+    const uint32_t split = blockIdx.x % a.nSplit;
+    const uint64_t row = blockIdx.x / a.nSplit;
+    const uint32_t from = static_cast<uint32_t>(static_cast<uint64_t>(a.vectors) * split / a.nSplit);
+    const uint32_t to = static_cast<uint32_t>(static_cast<uint64_t>(a.vectors) * (split + 1) / a.nSplit);
+    Token token = {a.nSplit == 1 ? TokenId(a, row) : -1, 0.0f};
+    if constexpr (kTop) {
+        for (uint32_t i = tid; i < kBins; i += kThreads) {
+            sh.bin[i] = 0;
         }
+        if (tid < kMaxTop) {
+            sh.top[tid] = 0;
+        }
+        if (tid == 0) {
+            sh.nGroups = 0;
+            sh.nCandidates = 0;
+        }
+    }
+    float largest;
+    bool any;
+    uint32_t nSlots;
+    Stats all = Pass<T, kThreads, kTop, false>(a, row, from, to, waveStats[0], waveMost, largest, any, groupMost, nSlots, token);
+    const float most = LaneMax(lane < kWaves ? waveMost[lane] : -__builtin_inff());     // of the workgroup
+    const bool safe = !(fabsf(most * a.exp2Scale) <= kReach);
+    if (safe) {
+        __syncthreads();      // (the maxima above are overwritten)
+        all = Pass<T, kThreads, kTop, true>(a, row, from, to, waveStats[1], waveMost, largest, any, groupMost, nSlots, token);
+    }
+    const RowResult result = Finish(all, safe, a);
+    if constexpr (kTop) {
+        if (!result.bad) {     // a NaN has no place in an order: no alternatives
+            GatherTop<T>(a, row, from, to, any ? Ordered(largest) : 0u, Ordered(most), nSlots, groupMost, sh, tid);
+        }
+    }
+    if (a.nSplit == 1) {
+        WriteRow<kThreads>(a, row, result, token, sh.top);
+        return;
+    }
+    const uint64_t at = row * a.nSplit + split;
+    if (tid == 0) {
+        StoreOne(a.stats + at * 4, all.m);
+        StoreOne(a.stats + at * 4 + 1, all.s);
+        StoreOne(a.stats + at * 4 + 2, all.t);
+        StoreOne(a.stats + at * 4 + 3, !safe ? 1.0f : most < 0.0f ? 0.0f : 2.0f);
     }
     if constexpr (kTop) {
-        if (result.bad) {     // a NaN has no place in an order: no alternatives
-            if (tid < a.topCount) {
-                if (a.nSplit == 1) {
-                    WriteTop(a, row, result, tid, 0);
-                } else {
-                    StoreOne(a.keys + (row * a.nSplit + split) * a.topCount + tid, static_cast<uint64_t>(0));
-                }
-            }
-            return;
-        }
-        __shared__ TopSpace sh;
-        const float most = acc.s == 0.0f ? -__builtin_inff() : acc.m;
-        GatherTop<T>(a, row, split, any ? Ordered(most) : 0u, sh, tid);
-        const uint32_t n = sh.nCandidates;
-        uint64_t* keys = a.keys + (row * a.nSplit + split) * a.topCount;
-        for (uint32_t c = tid; c < n; c += kThreads) {
-            const uint64_t key = sh.candidate[c];
-            uint32_t rank = 0;
-            for (uint32_t o = 0; o < n; ++o) {
-                rank += sh.candidate[o] > key ? 1 : 0;
-            }
-            if (rank < a.topCount) {
-                if (a.nSplit == 1) {
-                    WriteTop(a, row, result, rank, key);
-                } else {
-                    StoreOne(keys + rank, key);
-                }
-            }
-        }
-        if (a.nSplit > 1) {
-            for (uint32_t c = n + tid; c < a.topCount; c += kThreads) {
-                StoreOne(keys + c, static_cast<uint64_t>(0));
-            }
+        if (tid < a.topCount) {
+            StoreOne(a.keys + at * a.topCount + tid, result.bad ? 0 : sh.top[tid]);
         }
     }
 }
 
 // Joins the nSplit partial results of a row.
-constexpr uint32_t kMaxSplit = 64;
+constexpr uint32_t kJoinThreads = 256;
+constexpr uint32_t kMaxSplit = 32;
 template <typename T>
-__global__ __launch_bounds__(kThreads) void LogProbsJoinKernel(const LogProbsArgs a)
+__global__ __launch_bounds__(kJoinThreads) void LogProbsJoinKernel(const LogProbsArgs a)
 {
-    const uint32_t tid = threadIdx.x;
+    const uint32_t tid = threadIdx.x, lane = tid & (kWave - 1);
     const uint64_t row = blockIdx.x;
+    Token token = {TokenId(a, row), 0.0f};
     // every wavefront joins the numbers for itself, a lane per split
-    Stats mine = {kLowest, 0.0f, 0.0f};
-    const uint32_t lane = tid & (kWave - 1);
+    Stats mine = NoElements<false>();
+    float reach = -1.0f;    // 0, 1, 2: the split's largest logit is far below, within, far above what `m` can be a multiple of
+    const uint64_t* keys = a.keys + row * a.nSplit * a.topCount;
+    uint64_t last = 0;      // the lowest key of the lane's list
     if (lane < a.nSplit) {
         const float* p = a.stats + (row * a.nSplit + lane) * 4;
         mine = Stats{LoadOne(p), LoadOne(p + 1), LoadOne(p + 2)};
+        reach = mine.s != 0.0f ? LoadOne(p + 3) : -1.0f;
+        last = a.topCount != 0 ? LoadOne(keys + static_cast<uint64_t>(lane) * a.topCount + a.topCount - 1) : 0;
     }
-    const RowResult result = Finish(WaveJoin(mine, a.exp2Scale), a.scale);
-    if (tid == 0) {
-        WriteRow<T>(a, row, result);
+    token.logit = TokenLogit<T>(a, row, token.id);
+    // Splits of a lower class than the highest have no weight beside it (but a NaN in any shows).
+    const float highest = LaneMax(reach);
+    const bool safe = highest == 0.0f || highest == 2.0f, nan = __any(mine.s != mine.s);
+    if (reach != highest) {
+        mine = safe ? NoElements<true>() : NoElements<false>();
     }
+    Stats all = safe ? WaveJoin<true>(mine, a.exp2Scale) : WaveJoin<false>(mine, a.exp2Scale);
+    all.s = nan ? __builtin_nanf("") : all.s;
+    const RowResult result = Finish(all, safe, a);
+    __shared__ uint64_t top[kMaxTop];
+    if (a.topCount != 0 && !result.bad) {
+        // The largest topCount-th key of any list bounds the result from below: what is less drops out.
+        __shared__ uint64_t kept[kMaxSplit * kMaxTop];
+        __shared__ uint32_t nKept;
+        for (int d = 32; d > 0; d >>= 1) {
+            const uint64_t o = (static_cast<uint64_t>(__shfl_xor(static_cast<uint32_t>(last >> 32), d)) << 32) |
+                               __shfl_xor(static_cast<uint32_t>(last), d);
+            last = o > last ? o : last;
+        }
+        if (tid == 0) {
+            nKept = 0;
+        }
+        __syncthreads();
+        for (uint32_t c = tid; c < a.nSplit * a.topCount; c += kJoinThreads) {
+            const uint64_t key = LoadOne(keys + c);
+            if (key != 0 && key >= last) {
+                kept[atomicAdd(&nKept, 1u)] = key;
+            }
+        }
+        __syncthreads();
+        const uint32_t n = nKept;
+        for (uint32_t c = tid; c < n; c += kJoinThreads) {
+            const uint64_t key = kept[c];
+            const uint32_t rank = RankOf(key, kept, n);
+            if (rank < a.topCount) {
+                top[rank] = key;
+            }
+        }
+        __syncthreads();
+    }
+    WriteRow<kJoinThreads>(a, row, result, token, top);
+}
+
+template <typename T, uint32_t kThreads>
+void LaunchRows(LogProbsArgs& a, uint32_t rows, hipStream_t stream)
+{
+    const dim3 grid(rows * a.nSplit);
     if (a.topCount == 0) {
+        hipLaunchKernelGGL((LogProbsKernel<T, kThreads, false>), grid, dim3(kThreads), 0, stream, a);
         return;
     }
-    if (result.bad) {
-        if (tid < a.topCount) {
-            WriteTop(a, row, result, tid, 0);
-        }
-        return;
+    // Fetches of a workgroup: a short one at the end of every part, and no more than all parts' whole rows take.
+    constexpr uint32_t kFetch = kThreads * kUnroll;
+    uint32_t fetches = 0;
+    for (uint32_t s = 0; s < a.nShards; ++s) {
+        fetches += ((a.count[s] + kPer16<T> - 1) / kPer16<T> + kFetch - 1) / kFetch;
     }
-    // The largest topCount-th key of any list bounds the result from below: what is less drops out.
-    __shared__ uint64_t kept[kMaxSplit * kMaxTop];
-    __shared__ uint32_t nKept;
-    const uint64_t* keys = a.keys + row * a.nSplit * a.topCount;
-    uint64_t bound = lane < a.nSplit ? LoadOne(keys + static_cast<uint64_t>(lane) * a.topCount + a.topCount - 1) : 0;
-    for (int d = 32; d > 0; d >>= 1) {
-        const uint64_t o = (static_cast<uint64_t>(__shfl_xor(static_cast<uint32_t>(bound >> 32), d)) << 32) |
-                           __shfl_xor(static_cast<uint32_t>(bound), d);
-        bound = o > bound ? o : bound;
+    const uint32_t share = (a.vectors / a.nSplit + 1 + kFetch - 1) / kFetch + a.nShards;
+    fetches = fetches < share ? fetches : share;
+    a.slotShift = 0;
+    while (((fetches - 1) >> a.slotShift) + 1 > kGroupBytes / (kThreads * sizeof(uint16_t))) {
+        ++a.slotShift;
     }
-    if (tid == 0) {
-        nKept = 0;
-    }
-    __syncthreads();
-    for (uint32_t c = tid; c < a.nSplit * a.topCount; c += kThreads) {
-        const uint64_t key = LoadOne(keys + c);
-        if (key != 0 && key >= bound) {
-            kept[atomicAdd(&nKept, 1u)] = key;
-        }
-    }
-    __syncthreads();
-    const uint32_t n = nKept;
-    for (uint32_t c = tid; c < n; c += kThreads) {
-        const uint64_t key = kept[c];
-        uint32_t rank = 0;
-        for (uint32_t o = 0; o < n; ++o) {
-            rank += kept[o] > key ? 1 : 0;
-        }
-        if (rank < a.topCount) {
-            WriteTop(a, row, result, rank, key);
-        }
-    }
+    const uint32_t lds = (((fetches - 1) >> a.slotShift) + 1) * kThreads * sizeof(uint16_t);
+    hipLaunchKernelGGL((LogProbsKernel<T, kThreads, true>), grid, dim3(kThreads), lds, stream, a);
 }
 
 template <typename T>
-hipError_t Launch(const LogProbsArgs& a, uint32_t rows, hipStream_t stream)
+hipError_t Launch(LogProbsArgs& a, uint32_t rows, hipStream_t stream)
 {
-    const dim3 grid(rows * a.nSplit);
-    if (a.topCount != 0) {
-        hipLaunchKernelGGL((LogProbsKernel<T, true>), grid, dim3(kThreads), 0, stream, a);
-    } else {
-        hipLaunchKernelGGL((LogProbsKernel<T, false>), grid, dim3(kThreads), 0, stream, a);
+    switch (LogProbsFormOf(rows, a.vectors).threads) {
+        case 64: LaunchRows<T, 64>(a, rows, stream); break;
+        case 256: LaunchRows<T, 256>(a, rows, stream); break;
+        default: LaunchRows<T, 1024>(a, rows, stream); break;
     }
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && a.nSplit > 1) {
-        hipLaunchKernelGGL((LogProbsJoinKernel<T>), dim3(rows), dim3(kThreads), 0, stream, a);
+        hipLaunchKernelGGL((LogProbsJoinKernel<T>), dim3(rows), dim3(kJoinThreads), 0, stream, a);
         e = hipGetLastError();
     }
     return e;
@@ -597,17 +854,39 @@ hipError_t Launch(const LogProbsArgs& a, uint32_t rows, hipStream_t stream)
 
 }  // namespace
 
-// Few rows: as many workgroups per row as bring 1024 in all, each with at least 4096 elements.
-uint32_t LogProbsSplit(uint64_t rows, uint64_t vocab)
+// Measured on MI355X with bf16 rows, no alternatives / eight alternatives, in us (V = 8 vectors):
+//   rows x V        wave / row      256 / row       1024 / row      256, row split in
+//   4096 x 1000      7.4 / 11.5     17.6 / 25.1     71.6 / 122
+//   4096 x 16000    27.9 / 33.4     33.1 / 37.7     84.5 / 140
+//   4096 x 65536    89.5 / 97.4     88.8 / 93.7      117 / 175
+//   1024 x 4000      7.0 / 10.1      7.5 / 11.1     20.2 / 33.0
+//   1024 x 8000      9.4 / 12.8      8.6 / 12.1     21.9 / 35.7
+//    512 x 131072   69.1 / 78.1     27.0 / 31.7     29.6 / 37.2     29.8 / 35.2 (2)
+//    256 x 32768    19.2 / 24.0      8.7 / 12.2      8.2 / 11.4     10.0 / 14.5 (2)
+//    256 x 131072   66.5 / 75.8     22.2 / 27.1     16.4 / 20.2     18.2 / 23.4 (4)
+//    128 x 131072   65.8 / 75.2     20.9 / 26.0     13.4 / 17.4     12.7 / 17.6 (4)
+//     64 x 16000    10.5 / 13.8      6.3 / 9.0       6.9 / 10.3      7.5 / 12.0 (4)
+//     64 x 65536    34.0 / 40.2     12.0 / 16.2      8.7 / 12.5      8.5 / 13.1 (8)
+//     64 x 131072   65.2 / 74.1     20.5 / 25.5     13.0 / 17.1      9.9 / 14.7 (8)
+//     16 x 65536    27.7 / 33.7     11.1 / 14.5      8.5 / 12.0      7.2 / 11.4 (8)
+//      1 x 131072   42.9 / 51.0     13.5 / 17.9     11.2 / 14.8      6.5 / 11.0 (16)
+// A split row costs a second kernel of about 3 us, a workgroup of 1024 threads has a CU to itself.
+LogProbsForm LogProbsFormOf(uint64_t rows, uint64_t vectors)
 {
-    const uint64_t wanted = rows == 0 ? 1 : (1024 + rows - 1) / rows;
-    uint64_t split = vocab / 4096;
-    split = split < wanted ? split : wanted;
-    split = split < kMaxSplit ? split : kMaxSplit;
-    return split < 1 ? 1 : static_cast<uint32_t>(split);
+    if (2 * vectors <= rows) {
+        return {64, 1};
+    }
+    if (rows > 256 || vectors <= 2048) {
+        return {256, 1};
+    }
+    if (rows <= 128 && vectors > (rows <= 32 ? 4096 : 8192)) {
+        const uint64_t most = vectors < 65536 ? 16 : 32, wanted = 512 / rows;
+        return {256, static_cast<uint32_t>(wanted < most ? wanted : most)};
+    }
+    return {1024, 1};
 }
 
-hipError_t LaunchLogProbs(const LogProbsArgs& a, HcclDataType dtype, uint32_t rows, hipStream_t stream)
+hipError_t LaunchLogProbs(LogProbsArgs& a, HcclDataType dtype, uint32_t rows, hipStream_t stream)
 {
     switch (dtype) {
         case HCCL_DATA_TYPE_FP32: return Launch<F32>(a, rows, stream);

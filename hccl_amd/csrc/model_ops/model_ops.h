@@ -20,12 +20,14 @@ struct LogProbsArgs {
     uint64_t rowStride[kMaxShards];     // elements
     uint32_t count[kMaxShards];         // elements of the part
     const void* tokens;
-    float* stats;           // nSplit > 1: [row][split][4] = max, sum, weighted sum, -
+    float* stats;           // nSplit > 1: [row][split][4] = reference, sum, weighted sum, class of the reference
     uint64_t* keys;         //             [row][split][topCount], descending, 0 where there is none
     uint32_t nShards;
     uint32_t nSplit;        // workgroups per row
     uint32_t vocab;
+    uint32_t vectors;       // 16-byte vectors of the row, a short one at the end of a part counted
     uint32_t topCount;
+    uint32_t slotShift;     // filled by the launcher, see there
     uint32_t wideTokens;    // tokens and topIds are 64-bit
     float scale;
     float exp2Scale;        // scale * log2(e)
@@ -40,14 +42,23 @@ struct LogProbsArgs {
 };
 static_assert(sizeof(LogProbsArgs) <= 4096, "kernel arguments");
 
-// Workgroups per row, from the sizes alone.
-uint32_t LogProbsSplit(uint64_t rows, uint64_t vocab);
+// 16-byte vectors of a part's row.
+inline uint64_t LogProbsVectors(uint64_t count, uint32_t elementSize) { return (count * elementSize + 15) / 16; }
+// How a call is launched, from its rows and the vectors of a row alone: threads per workgroup and workgroups per row.  More
+// vectors never mean fewer workgroups per row (LogProbsWorkspace relies on it).
+struct LogProbsForm {
+    uint32_t threads;
+    uint32_t split;
+};
+LogProbsForm LogProbsFormOf(uint64_t rows, uint64_t vectors);
+// Enough for every type and any parts: 32-bit elements, and a short vector at the end of each part.
 inline uint64_t LogProbsWorkspace(uint64_t rows, uint64_t vocab, uint32_t top)
 {
-    const uint64_t split = LogProbsSplit(rows, vocab);
+    const uint64_t split = rows == 0 ? 1 : LogProbsFormOf(rows, LogProbsVectors(vocab, 4) + kMaxShards).split;
     return split <= 1 ? 0 : rows * split * (4 * sizeof(float) + top * sizeof(uint64_t));
 }
-hipError_t LaunchLogProbs(const LogProbsArgs& args, HcclDataType dtype, uint32_t rows, hipStream_t stream);
+// args.vectors and args.nSplit are the form's.
+hipError_t LaunchLogProbs(LogProbsArgs& args, HcclDataType dtype, uint32_t rows, hipStream_t stream);
 
 // ---- their gradient ---------------------------------------------------------------------------------------------
 struct LogProbsGradArgs {

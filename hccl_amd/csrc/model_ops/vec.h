@@ -18,12 +18,15 @@ constexpr uint32_t kWave = 64;
 
 struct F32 {
     typedef uint32_t Raw;
+    static constexpr bool kHalf = false;
 };
 struct B16 {
     typedef uint16_t Raw;
+    static constexpr bool kHalf = false;
 };
 struct F16 {
     typedef uint16_t Raw;
+    static constexpr bool kHalf = true;
 };
 
 template <typename T>
@@ -128,25 +131,97 @@ __device__ __forceinline__ void StoreOne(V* p, V v)
     *((HCCL_AMD_GLOBAL V*)p) = v;
 }
 
-__device__ __forceinline__ float WaveMax(float v)
+// The value of lane (lane ^ D), for D a power of two, without LDS: permutations within four and sixteen lanes that the
+// vector ALU applies to an operand, and the exchanges of 16- and 32-lane rows.
+template <int kControl>
+__device__ __forceinline__ uint32_t Dpp(uint32_t v)
 {
-    for (int d = 32; d > 0; d >>= 1) {
-        v = fmaxf(v, __shfl_xor(v, d));
+    return __builtin_amdgcn_update_dpp(0, v, kControl, 0xF, 0xF, true);
+}
+constexpr int kQuadXor1 = 0xB1, kQuadXor2 = 0x4E, kQuadXor3 = 0x1B, kHalfMirror = 0x141, kMirror = 0x140, kRotate8 = 0x128;
+
+// Both values of a pair of lanes 16 or 32 apart: x is the lower lane's, y the upper lane's, on both.
+template <uint32_t D>
+__device__ __forceinline__ U32x2 RowPair(uint32_t v)
+{
+    if constexpr (D == 16) {
+        return __builtin_bit_cast(U32x2, __builtin_amdgcn_permlane16_swap(v, v, false, false));
+    } else {
+        return __builtin_bit_cast(U32x2, __builtin_amdgcn_permlane32_swap(v, v, false, false));
+    }
+}
+
+template <uint32_t D>
+__device__ __forceinline__ uint32_t XorLane(uint32_t v)
+{
+    if constexpr (D == 1) {
+        return Dpp<kQuadXor1>(v);
+    } else if constexpr (D == 2) {
+        return Dpp<kQuadXor2>(v);
+    } else if constexpr (D == 4) {
+        return Dpp<kQuadXor3>(Dpp<kHalfMirror>(v));     // 7 ^ 3
+    } else if constexpr (D == 8) {
+        return Dpp<kRotate8>(v);
+    } else {
+        const U32x2 pair = RowPair<D>(v);
+        return (threadIdx.x & D) == 0 ? pair.y : pair.x;
+    }
+}
+template <uint32_t D>
+__device__ __forceinline__ float XorLane(float v)
+{
+    return __builtin_bit_cast(float, XorLane<D>(__builtin_bit_cast(uint32_t, v)));
+}
+template <uint32_t D>
+__device__ __forceinline__ double XorLane(double v)
+{
+    const U32x2 w = __builtin_bit_cast(U32x2, v);
+    return __builtin_bit_cast(double, U32x2{XorLane<D>(w.x), XorLane<D>(w.y)});
+}
+
+// Reductions over groups of kLanes neighbouring lanes; every lane gets the result, and all the same bits (the operands of
+// a pair only change places).
+template <uint32_t kLanes = kWave>
+__device__ __forceinline__ float LaneMax(float v)
+{
+    v = fmaxf(v, XorLane<1>(v));
+    v = fmaxf(v, XorLane<2>(v));
+    v = fmaxf(v, XorLane<4>(v));
+    v = fmaxf(v, XorLane<8>(v));
+    if constexpr (kLanes >= 32) {
+        v = fmaxf(v, XorLane<16>(v));
+    }
+    if constexpr (kLanes >= 64) {
+        v = fmaxf(v, XorLane<32>(v));
     }
     return v;
 }
-__device__ __forceinline__ float WaveSum(float v)
+template <typename V>
+__device__ __forceinline__ V WaveSum(V v)
 {
-    for (int d = 32; d > 0; d >>= 1) {
-        v += __shfl_xor(v, d);
-    }
+    v += XorLane<1>(v);
+    v += XorLane<2>(v);
+    v += XorLane<4>(v);
+    v += XorLane<8>(v);
+    v += XorLane<16>(v);
+    v += XorLane<32>(v);
     return v;
 }
-__device__ __forceinline__ double WaveSum(double v)
+
+// Sum over the lanes up to and including the own one.
+template <int kControl, int kRows>
+__device__ __forceinline__ uint32_t FromLower(uint32_t v)
 {
-    for (int d = 32; d > 0; d >>= 1) {
-        v += __shfl_xor(v, d);
-    }
+    return __builtin_amdgcn_update_dpp(0, v, kControl, kRows, 0xF, false);      // 0 where there is no such lane
+}
+__device__ __forceinline__ uint32_t WaveScan(uint32_t v)
+{
+    v += FromLower<0x111, 0xF>(v);      // shifts by 1, 2, 4, 8 within sixteen lanes
+    v += FromLower<0x112, 0xF>(v);
+    v += FromLower<0x114, 0xF>(v);
+    v += FromLower<0x118, 0xF>(v);
+    v += FromLower<0x142, 0xA>(v);      // the last lane of rows 0 and 2 to rows 1 and 3
+    v += FromLower<0x143, 0xC>(v);      // lane 31 to the upper half
     return v;
 }
 

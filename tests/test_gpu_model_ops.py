@@ -235,6 +235,31 @@ def test_many_equal_logits(worlds, t, v):
     check_rows(rows, rows.run(worlds(1), tokens), tokens, 1.0)
 
 
+@pytest.mark.parametrize("t,threads", [(129, 1024), (257, 256)])
+def test_more_large_logits_in_one_lane_than_its_list_takes(worlds, t, threads):
+    """Columns that one lane of a workgroup reads hold all the large values, rising, beside a row of zeros: the alternatives
+    are the last of them, found by bisection.  (The lane map is the kernel's; with another one the case is an easy one.)"""
+    v = 4 * threads * 600
+    w = worlds(1)
+    x = torch.zeros(t, v, device="cuda")
+    column = torch.arange(v, device="cuda")
+    columns = column[(column // 4) % threads == 7]
+    x[0, columns] = 1 + torch.arange(len(columns), device="cuda") / 4096
+    x[1, columns] = 1 + torch.arange(len(columns), device="cuda").flip(0) / 4096
+    values = torch.zeros(t, 32, device="cuda")
+    ids = torch.zeros(t, 32, device="cuda", dtype=torch.int64)
+    torch.cuda.synchronize()
+    model_ops.token_log_probs(w.comms[0], x, t, 0, v, None, None, data_type=DT.FP32, top_count=32, top_values=values,
+                              top_ids=ids, stream=w.stream)
+    w.sync()
+    assert ids[0].tolist() == columns.flip(0)[:32].tolist()
+    assert ids[1].tolist() == columns[:32].tolist()
+    assert ids[2].tolist() == list(range(32))
+    for row in range(3):
+        want = torch.log_softmax(x[row].double(), 0)[ids[row]]
+        assert float((values[row].double() - want).abs().max()) <= (terms(v) + 8 + 64) * U
+
+
 def test_outputs_are_optional_and_each_may_go_elsewhere(worlds):
     x = rng_tensor(3, 40, 999)
     tokens = given(40, 999, 2)
