@@ -1,12 +1,16 @@
 // One AdamW step over a batch of tensors, states in 32 bits or as e4m3 codes with a scale per 256 elements.
 //
-// Purely elementwise but for the scales.  A lane owns eight neighbouring elements, a wavefront 512, so that a block of 256
-// is half a wavefront: its largest magnitude takes five exchanges between lanes and no memory.  m and v are updated in
-// 32 bits and rounded once on the way out; the weights take the unrounded ones.  Of v the root is stored: that halves the
-// exponents it needs, and it is what the step divides by.  A root above zero is stored as at least the smallest code:
-// rounded to zero it would leave m / eps as a step.
+// Purely elementwise but for the scales.  A lane owns four neighbouring elements, 16 bytes of a 32-bit tensor, so that every
+// access of a wavefront is one run of memory, and a wavefront owns a state block of 256: its largest magnitude takes six
+// exchanges between lanes and no memory.  m and v are updated in 32 bits and rounded once on the way out; the weights take
+// the unrounded ones.  Of v the root is stored: that halves the exponents it needs, and it is what the step divides by.  A
+// root above zero is stored as at least the smallest code: rounded to zero it would leave m / eps as a step.
 // Square root and reciprocal are the one-instruction forms (1 ulp): the step is 1e-7 of itself off, the weight far less.
-// Bound: every tensor read once and the updated ones written once.
+//
+// Bound: every tensor read once and the updated ones written once.  2^27 bf16 weights in 300 tensors with 32-bit master
+// weights, four launches: 629 us, 6.0 TB/s of the 6.0 - 6.7 that a copy reaches; with FP8 states 379 us, 5.7 TB/s.  (A lane
+// with eight neighbours, two 16-byte accesses 32 bytes apart: 790 and 486.  Chunks of 1024 elements 631 and 393, of 4096
+// 676 and 396; stores written through 651 and 391, plain ones 701 and 414.)
 #include "model_ops.h"
 #include "vec.h"
 
@@ -15,25 +19,30 @@ namespace model_ops {
 namespace {
 
 constexpr uint32_t kThreads = 256;
-constexpr uint32_t kPer = 8;                                   // elements of a lane
+constexpr uint32_t kPer = 4;                                   // elements of a lane
 constexpr uint32_t kSteps = kAdamWChunk / (kThreads * kPer);   // per workgroup
 constexpr uint32_t kBlock = HCCL_AMD_STATE_BLOCK;
-constexpr uint32_t kBlockLanes = kBlock / kPer;
 constexpr float kCodeMax = 448.0f;           // largest e4m3 value
 constexpr float kCodeMin = 0.001953125f;     // smallest above 0
 constexpr float kNoUnit = 1e-35f;            // below it 448 / x is beyond a float: such a block counts as zero
-static_assert(kBlockLanes == 32 && kAdamWChunk % kBlock == 0, "a block is half a wavefront and never leaves its chunk");
+static_assert(kBlock == kWave * kPer && kAdamWChunk % kBlock == 0, "a block is a wavefront and never leaves its chunk");
 
-// Eight elements from element `at`, which has `n` (1 .. 8) left in the tensor.
+// Four elements from element `at`, of which `n` (0 .. 4, or more) are in the tensor; the others are 0.
 template <typename T>
-__device__ __forceinline__ void Load8(const void* base, uint64_t at, uint32_t n, float* x)
+__device__ __forceinline__ void Load4(uint64_t base, uint64_t at, uint32_t n, float* x)
 {
     typedef typename T::Raw Raw;
-    const Raw* p = static_cast<const Raw*>(base) + at;
+    const Raw* p = reinterpret_cast<const Raw*>(base) + at;
     if (n >= kPer) {
-        Unpack16<T>(LoadOnce16(p), x);
         if constexpr (sizeof(Raw) == 4) {
-            Unpack16<T>(LoadOnce16(p + 4), x + 4);
+            Unpack16<T>(LoadOnce16(p), x);
+        } else {
+            const U32x2 raw = LoadOnce8(p);
+            for (uint32_t i = 0; i < 2; ++i) {
+                const uint32_t word = raw[i];
+                x[2 * i] = Widen<T>(static_cast<uint16_t>(word & 0xFFFFu));
+                x[2 * i + 1] = Widen<T>(static_cast<uint16_t>(word >> 16));
+            }
         }
     } else {
         for (uint32_t i = 0; i < kPer; ++i) {
@@ -43,14 +52,19 @@ __device__ __forceinline__ void Load8(const void* base, uint64_t at, uint32_t n,
 }
 
 template <typename T>
-__device__ __forceinline__ void Store8(void* base, uint64_t at, uint32_t n, const float* x)
+__device__ __forceinline__ void Store4(uint64_t base, uint64_t at, uint32_t n, const float* x)
 {
     typedef typename T::Raw Raw;
-    Raw* p = static_cast<Raw*>(base) + at;
+    Raw* p = reinterpret_cast<Raw*>(base) + at;
     if (n >= kPer) {
-        StoreOnce16(p, Pack16<T>(x));
         if constexpr (sizeof(Raw) == 4) {
-            StoreOnce16(p + 4, Pack16<T>(x + 4));
+            StoreOnce16(p, Pack16<T>(x));
+        } else {
+            U32x2 raw;
+            for (uint32_t i = 0; i < 2; ++i) {
+                raw[i] = static_cast<uint32_t>(Narrow<T>(x[2 * i])) | (static_cast<uint32_t>(Narrow<T>(x[2 * i + 1])) << 16);
+            }
+            StoreOnce8(p, raw);
         }
     } else {
         for (uint32_t i = 0; i < kPer; ++i) {
@@ -61,62 +75,97 @@ __device__ __forceinline__ void Store8(void* base, uint64_t at, uint32_t n, cons
     }
 }
 
-__device__ __forceinline__ void LoadCodes(const void* base, uint64_t at, uint32_t n, float* x)
+typedef uint32_t CodesAny __attribute__((aligned(1)));
+__device__ __forceinline__ uint32_t LoadCodes(uint64_t base, uint64_t at, uint32_t n)
 {
-    const uint8_t* p = static_cast<const uint8_t*>(base) + at;
-    U32x2 raw = {0, 0};
+    const uint8_t* p = reinterpret_cast<const uint8_t*>(base) + at;
     if (n >= kPer) {
-        raw = LoadOnce8(p);
-    } else {
-        for (uint32_t i = 0; i < kPer; ++i) {
-            const uint32_t code = i < n ? LoadOne(p + i) : 0;
-            raw[i / 4] |= code << (8 * (i % 4));
-        }
+        return __builtin_nontemporal_load((const HCCL_AMD_GLOBAL CodesAny*)p);
     }
-    for (uint32_t w = 0; w < 2; ++w) {
-        x[4 * w] = __builtin_amdgcn_cvt_f32_fp8(raw[w], 0);
-        x[4 * w + 1] = __builtin_amdgcn_cvt_f32_fp8(raw[w], 1);
-        x[4 * w + 2] = __builtin_amdgcn_cvt_f32_fp8(raw[w], 2);
-        x[4 * w + 3] = __builtin_amdgcn_cvt_f32_fp8(raw[w], 3);
+    uint32_t codes = 0;
+    for (uint32_t i = 0; i < kPer; ++i) {
+        codes |= i < n ? static_cast<uint32_t>(LoadOne(p + i)) << (8 * i) : 0u;
     }
+    return codes;
 }
 
-__device__ __forceinline__ void StoreCodes(void* base, uint64_t at, uint32_t n, const float* x)
+__device__ __forceinline__ void Decode(uint32_t codes, float scale, float* x)
 {
-    uint8_t* p = static_cast<uint8_t*>(base) + at;
-    U32x2 raw;
-    for (uint32_t w = 0; w < 2; ++w) {
-        int packed = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * w], x[4 * w + 1], 0, false);
-        packed = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * w + 2], x[4 * w + 3], packed, true);
-        raw[w] = static_cast<uint32_t>(packed);
-    }
+    x[0] = scale * __builtin_amdgcn_cvt_f32_fp8(codes, 0);
+    x[1] = scale * __builtin_amdgcn_cvt_f32_fp8(codes, 1);
+    x[2] = scale * __builtin_amdgcn_cvt_f32_fp8(codes, 2);
+    x[3] = scale * __builtin_amdgcn_cvt_f32_fp8(codes, 3);
+}
+
+__device__ __forceinline__ void StoreCodes(uint64_t base, uint64_t at, uint32_t n, const float* x)
+{
+    uint8_t* p = reinterpret_cast<uint8_t*>(base) + at;
+    int packed = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+    packed = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], packed, true);
+    const uint32_t codes = static_cast<uint32_t>(packed);
     if (n >= kPer) {
-        StoreOnce8(p, raw);
+        __builtin_nontemporal_store(codes, (HCCL_AMD_GLOBAL CodesAny*)p);
     } else {
         for (uint32_t i = 0; i < kPer; ++i) {
             if (i < n) {
-                StoreOne(p + i, static_cast<uint8_t>(raw[i / 4] >> (8 * (i % 4))));
+                StoreOne(p + i, static_cast<uint8_t>(codes >> (8 * i)));
             }
         }
     }
 }
 
-// Largest of the eight magnitudes over the 32 lanes of a block.
+// Largest magnitude of a block.
 __device__ __forceinline__ float BlockMax(const float* x)
 {
-    float most = fabsf(x[0]);
-    for (uint32_t i = 1; i < kPer; ++i) {
-        most = fmaxf(most, fabsf(x[i]));
-    }
-    for (uint32_t d = kBlockLanes / 2; d > 0; d >>= 1) {
-        most = fmaxf(most, __shfl_xor(most, d));
-    }
-    return most;
+    return LaneMax(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
 }
 
 template <typename P, typename G, bool kMaster, bool kFp8>
 __global__ __launch_bounds__(kThreads) void AdamWKernel(const AdamWArgs a)
 {
+    constexpr uint32_t kStride = AdamWTensorWords(kMaster, kFp8);
+    uint32_t lo = 0, hi = a.nTensors - 1;      // the first tensor that ends behind this chunk
+    while (lo < hi) {
+        const uint32_t mid = (lo + hi) / 2;
+        if (static_cast<uint32_t>(a.table[mid * kStride]) > blockIdx.x) {
+            hi = mid;
+        } else {
+            lo = mid + 1;
+        }
+    }
+    const uint64_t* t = a.table + lo * kStride;
+    const uint32_t chunk = blockIdx.x - (lo == 0 ? 0u : static_cast<uint32_t>(a.table[(lo - 1) * kStride]));
+    const uint64_t begin = static_cast<uint64_t>(chunk) * kAdamWChunk;
+    const uint32_t inChunk = blockIdx.x + 1 == static_cast<uint32_t>(t[0]) ? static_cast<uint32_t>(t[0] >> 32) : kAdamWChunk;
+    const uint64_t param = t[1], grad = t[2], expAvg = t[3], expAvgSq = t[4];
+    const uint64_t weights = kMaster ? t[5] : param;
+    float* const mScales = kFp8 ? reinterpret_cast<float*>(t[kStride - 2]) : nullptr;
+    float* const vScales = kFp8 ? reinterpret_cast<float*>(t[kStride - 1]) : nullptr;
+
+    // everything is on its way before the step's numbers are
+    float w[kSteps][kPer], g[kSteps][kPer], m[kSteps][kPer], v[kSteps][kPer], mScale[kSteps], vScale[kSteps];
+    uint32_t mCodes[kSteps], vCodes[kSteps];
+    for (uint32_t s = 0; s < kSteps; ++s) {
+        const uint32_t off = (s * kThreads + threadIdx.x) * kPer;
+        const uint64_t at = begin + off;
+        const uint32_t n = off < inChunk ? inChunk - off : 0;
+        if constexpr (kMaster) {
+            Load4<F32>(weights, at, n, w[s]);
+        } else {
+            Load4<P>(weights, at, n, w[s]);
+        }
+        Load4<G>(grad, at, n, g[s]);
+        if constexpr (kFp8) {
+            mCodes[s] = LoadCodes(expAvg, at, n);
+            vCodes[s] = LoadCodes(expAvgSq, at, n);
+            mScale[s] = n != 0 ? LoadOne(mScales + at / kBlock) : 0.0f;
+            vScale[s] = n != 0 ? LoadOne(vScales + at / kBlock) : 0.0f;
+        } else {
+            Load4<F32>(expAvg, at, n, m[s]);
+            Load4<F32>(expAvgSq, at, n, v[s]);
+        }
+    }
+
     float clip = 1.0f;
     if (a.clip != nullptr) {
         if (a.skipNonFinite && !(fabsf(LoadOne(a.clip)) < __builtin_inff())) {
@@ -133,89 +182,59 @@ __global__ __launch_bounds__(kThreads) void AdamWKernel(const AdamWArgs a)
     }
     const float rate = lr * correction1, keep = 1.0f - lr * a.weightDecay;
 
-    uint32_t lo = 0, hi = a.nTensors - 1;      // the first tensor that ends behind this chunk
-    while (lo < hi) {
-        const uint32_t mid = (lo + hi) / 2;
-        if (a.chunkEnd[mid] > blockIdx.x) {
-            hi = mid;
-        } else {
-            lo = mid + 1;
-        }
-    }
-    const AdamWArgs::Tensor& t = a.t[lo];
-    const uint64_t begin = static_cast<uint64_t>(blockIdx.x - (lo == 0 ? 0 : a.chunkEnd[lo - 1])) * kAdamWChunk;
-    const uint64_t left = t.count - begin;
-    const uint32_t inChunk = left < kAdamWChunk ? static_cast<uint32_t>(left) : kAdamWChunk;
-
     for (uint32_t s = 0; s < kSteps; ++s) {
         const uint32_t off = (s * kThreads + threadIdx.x) * kPer;
         const uint64_t at = begin + off;
         const uint32_t n = off < inChunk ? inChunk - off : 0;
-        float w[kPer], g[kPer], m[kPer], v[kPer];
-        float mScale = 0.0f, vScale = 0.0f;
-        if (n != 0) {
-            if constexpr (kMaster) {
-                Load8<F32>(t.master, at, n, w);
-            } else {
-                Load8<P>(t.param, at, n, w);
-            }
-            Load8<G>(t.grad, at, n, g);
-            if constexpr (kFp8) {
-                LoadCodes(t.m, at, n, m);
-                LoadCodes(t.v, at, n, v);
-                mScale = LoadOne(t.mScale + at / kBlock);
-                vScale = LoadOne(t.vScale + at / kBlock);
-            } else {
-                Load8<F32>(t.m, at, n, m);
-                Load8<F32>(t.v, at, n, v);
-            }
-        } else {
-            for (uint32_t i = 0; i < kPer; ++i) {
-                w[i] = g[i] = m[i] = v[i] = 0.0f;
-            }
+        if constexpr (kFp8) {
+            Decode(mCodes[s], mScale[s], m[s]);
+            Decode(vCodes[s], vScale[s], v[s]);
         }
         float root[kPer];
         for (uint32_t i = 0; i < kPer; ++i) {
             if constexpr (kFp8) {
-                m[i] *= mScale;
-                v[i] *= vScale;
-                v[i] *= v[i];
+                v[s][i] *= v[s][i];
             }
-            const float gi = g[i] * clip;
-            m[i] = __builtin_fmaf(m[i], a.beta1, gi * a.oneMinusBeta1);
-            v[i] = __builtin_fmaf(v[i], a.beta2, gi * gi * a.oneMinusBeta2);
-            root[i] = __builtin_amdgcn_sqrtf(v[i]);
-            const float step = m[i] * __builtin_amdgcn_rcpf(__builtin_fmaf(root[i], rootCorrection2, a.eps));
-            w[i] = __builtin_fmaf(-rate, step, w[i] * keep);
+            const float gi = g[s][i] * clip;
+            m[s][i] = __builtin_fmaf(m[s][i], a.beta1, gi * a.oneMinusBeta1);
+            v[s][i] = __builtin_fmaf(v[s][i], a.beta2, gi * gi * a.oneMinusBeta2);
+            root[i] = __builtin_amdgcn_sqrtf(v[s][i]);
+            const float step = m[s][i] * __builtin_amdgcn_rcpf(__builtin_fmaf(root[i], rootCorrection2, a.eps));
+            w[s][i] = __builtin_fmaf(-rate, step, w[s][i] * keep);
             if constexpr (kMaster) {
                 // The 16-bit weights are the rounded master weights: without this the compiler rounds the fused
                 // multiply-add to 16 bits in one instruction, past the 32-bit value.
-                asm("" : "+v"(w[i]));
+                asm("" : "+v"(w[s][i]));
             }
         }
         if constexpr (kFp8) {
-            const float mMost = BlockMax(m), vMost = BlockMax(root);
+            // (places behind the tensor's end have zeros)
+            for (uint32_t i = 0; i < kPer; ++i) {
+                m[s][i] = i < n ? m[s][i] : 0.0f;
+                root[i] = i < n ? root[i] : 0.0f;
+            }
+            const float mMost = BlockMax(m[s]), vMost = BlockMax(root);
             const float mUnit = mMost > kNoUnit ? kCodeMax / mMost : 0.0f, vUnit = vMost > kNoUnit ? kCodeMax / vMost : 0.0f;
             for (uint32_t i = 0; i < kPer; ++i) {
-                m[i] *= mUnit;
+                m[s][i] *= mUnit;
                 root[i] = root[i] > 0.0f ? fmaxf(root[i] * vUnit, kCodeMin) : root[i];
             }
-            if (n != 0 && threadIdx.x % kBlockLanes == 0) {
-                StoreOne(t.mScale + at / kBlock, mMost / kCodeMax);
-                StoreOne(t.vScale + at / kBlock, vMost / kCodeMax);
+            if (n != 0 && threadIdx.x % kWave == 0) {
+                StoreOne(mScales + at / kBlock, mMost / kCodeMax);
+                StoreOne(vScales + at / kBlock, vMost / kCodeMax);
             }
         }
         if (n != 0) {
-            Store8<P>(t.param, at, n, w);
+            Store4<P>(param, at, n, w[s]);
             if constexpr (kMaster) {
-                Store8<F32>(t.master, at, n, w);
+                Store4<F32>(weights, at, n, w[s]);
             }
             if constexpr (kFp8) {
-                StoreCodes(t.m, at, n, m);
-                StoreCodes(t.v, at, n, root);
+                StoreCodes(expAvg, at, n, m[s]);
+                StoreCodes(expAvgSq, at, n, root);
             } else {
-                Store8<F32>(t.m, at, n, m);
-                Store8<F32>(t.v, at, n, v);
+                Store4<F32>(expAvg, at, n, m[s]);
+                Store4<F32>(expAvgSq, at, n, v[s]);
             }
         }
     }

@@ -204,18 +204,25 @@ HcclResult RunGradNorm(World* w, PendingOp& p, hipStream_t s)
     join.scale = calls[0].scale;
     join.nOut = w->n;
     NormArgs a = {};
+    uint32_t nTensors = 0;
     const auto flush = [&]() -> HcclResult {
         if (a.nChunks != 0) {
             if ((join.nPartial + kNormGroups) * sizeof(double) > need) {
                 return HCCL_E_INTERNAL;
             }
-            a.perGroup = (a.nChunks + kNormGroups - 1) / kNormGroups;
             a.partial = partial + join.nPartial;
+            a.perGroup = (a.nChunks + kNormGroups - 1) / kNormGroups;
             const uint32_t groups = (a.nChunks + a.perGroup - 1) / a.perGroup;
+            for (uint32_t i = nTensors; i < kNormBatch; ++i) {
+                a.chunkEnd[i] = 0xFFFFFFFFu;
+            }
+            for (uint32_t i = 0; i < 16; ++i) {
+                a.groupEnd[i] = i < kNormBatch / 16 ? a.chunkEnd[16 * i + 15] : 0xFFFFFFFFu;
+            }
             HIP_OK(LaunchNormBatch(a, groups, s));
             join.nPartial += groups;
         }
-        a.nTensors = a.nChunks = 0;
+        nTensors = a.nChunks = 0;
         return HCCL_SUCCESS;
     };
     for (uint32_t r = 0; r < w->n; ++r) {
@@ -227,18 +234,18 @@ HcclResult RunGradNorm(World* w, PendingOp& p, hipStream_t s)
             if (chunks == 0) {
                 continue;
             }
-            if (a.nTensors == kNormBatch || a.nChunks + chunks > kMaxChunks) {
+            if (nTensors == kNormBatch || a.nChunks + chunks > kMaxChunks) {
                 HcclResult rc = flush();
                 if (rc != HCCL_SUCCESS) {
                     return rc;
                 }
             }
             a.nChunks += static_cast<uint32_t>(chunks);
-            a.data[a.nTensors] = reinterpret_cast<const void*>(d[0]);
-            a.chunkEnd[a.nTensors] = a.nChunks;
-            a.lastChunk[a.nTensors] = static_cast<uint32_t>(d[1] - (chunks - 1) * perChunk) << 2 |
-                                      (type == HCCL_DATA_TYPE_FP32 ? 0u : type == HCCL_DATA_TYPE_BFP16 ? 1u : 2u);
-            a.nTensors++;
+            a.data[nTensors] = reinterpret_cast<const void*>(d[0]);
+            a.chunkEnd[nTensors] = a.nChunks;
+            a.lastChunk[nTensors] = static_cast<uint32_t>((d[1] - (chunks - 1) * perChunk) * DataTypeSize(type)) << 2 |
+                                    (type == HCCL_DATA_TYPE_FP32 ? 0u : type == HCCL_DATA_TYPE_BFP16 ? 1u : 2u);
+            nTensors++;
         }
     }
     HcclResult rc = flush();
@@ -386,6 +393,8 @@ HcclResult CheckAdamWConfig(const char* name, const HcclAmdAdamWConfig& c)
     return HCCL_SUCCESS;
 }
 
+constexpr uint32_t kMaxAdamWChunks = 1u << 23;
+
 // Tensors of one combination of types, in batches.
 HcclResult RunAdamW(const HcclAmdAdamWTensor* tensors, uint32_t tensorCount, AdamWArgs& a, bool fp8, hipStream_t s)
 {
@@ -395,11 +404,13 @@ HcclResult RunAdamW(const HcclAmdAdamWTensor* tensors, uint32_t tensorCount, Ada
             continue;
         }
         const HcclAmdAdamWTensor& like = tensors[i];
+        const bool master = like.master != nullptr;
+        const uint32_t stride = AdamWTensorWords(master, fp8);
         uint32_t chunks = 0;
         a.nTensors = 0;
         const auto flush = [&]() -> HcclResult {
             if (chunks != 0) {
-                HIP_OK(LaunchAdamW(a, like.paramType, like.gradType, like.master != nullptr, fp8, chunks, s));
+                HIP_OK(LaunchAdamW(a, like.paramType, like.gradType, master, fp8, chunks, s));
             }
             chunks = a.nTensors = 0;
             return HCCL_SUCCESS;
@@ -407,32 +418,36 @@ HcclResult RunAdamW(const HcclAmdAdamWTensor* tensors, uint32_t tensorCount, Ada
         for (uint32_t j = i; j < tensorCount; ++j) {
             const HcclAmdAdamWTensor& t = tensors[j];
             if (done[j] || t.count == 0 || t.paramType != like.paramType || t.gradType != like.gradType ||
-                (t.master != nullptr) != (like.master != nullptr)) {
+                (t.master != nullptr) != master) {
                 continue;
             }
             done[j] = 1;
+            const uint64_t ps = DataTypeSize(t.paramType), gs = DataTypeSize(t.gradType), ss = fp8 ? 1 : 4;
             // A launch has fewer than 2^32 work items: a tensor of more than 2^23 chunks takes several pieces.
             for (uint64_t at = 0; at < t.count;) {
-                if (a.nTensors == kAdamWBatch || chunks == 1u << 23) {
+                if ((a.nTensors + 1) * stride > kAdamWWords || chunks == kMaxAdamWChunks) {
                     HcclResult rc = flush();
                     if (rc != HCCL_SUCCESS) {
                         return rc;
                     }
                 }
-                const uint64_t room = static_cast<uint64_t>((1u << 23) - chunks) * kAdamWChunk;
+                const uint64_t room = static_cast<uint64_t>(kMaxAdamWChunks - chunks) * kAdamWChunk;
                 const uint64_t n = t.count - at < room ? t.count - at : room;
-                const uint64_t ps = DataTypeSize(t.paramType), gs = DataTypeSize(t.gradType), ss = fp8 ? 1 : 4;
-                AdamWArgs::Tensor& d = a.t[a.nTensors];
-                d.param = static_cast<uint8_t*>(t.param) + at * ps;
-                d.grad = static_cast<const uint8_t*>(t.grad) + at * gs;
-                d.m = static_cast<uint8_t*>(t.expAvg) + at * ss;
-                d.v = static_cast<uint8_t*>(t.expAvgSq) + at * ss;
-                d.master = t.master != nullptr ? t.master + at : nullptr;
-                d.mScale = fp8 ? t.expAvgScale + at / HCCL_AMD_STATE_BLOCK : nullptr;
-                d.vScale = fp8 ? t.expAvgSqScale + at / HCCL_AMD_STATE_BLOCK : nullptr;
-                d.count = n;
-                chunks += static_cast<uint32_t>((n + kAdamWChunk - 1) / kAdamWChunk);
-                a.chunkEnd[a.nTensors++] = chunks;
+                const uint64_t mine = (n + kAdamWChunk - 1) / kAdamWChunk;
+                chunks += static_cast<uint32_t>(mine);
+                uint64_t* d = a.table + static_cast<size_t>(a.nTensors++) * stride;
+                *d++ = chunks | (n - (mine - 1) * kAdamWChunk) << 32;
+                *d++ = reinterpret_cast<uint64_t>(t.param) + at * ps;
+                *d++ = reinterpret_cast<uint64_t>(t.grad) + at * gs;
+                *d++ = reinterpret_cast<uint64_t>(t.expAvg) + at * ss;
+                *d++ = reinterpret_cast<uint64_t>(t.expAvgSq) + at * ss;
+                if (master) {
+                    *d++ = reinterpret_cast<uint64_t>(t.master + at);
+                }
+                if (fp8) {
+                    *d++ = reinterpret_cast<uint64_t>(t.expAvgScale + at / HCCL_AMD_STATE_BLOCK);
+                    *d++ = reinterpret_cast<uint64_t>(t.expAvgSqScale + at / HCCL_AMD_STATE_BLOCK);
+                }
                 at += n;
             }
         }

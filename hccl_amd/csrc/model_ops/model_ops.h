@@ -83,19 +83,19 @@ hipError_t LaunchLogProbsGrad(const LogProbsGradArgs& args, HcclDataType dtype, 
 
 // ---- gradient norm ------------------------------------------------------------------------------------------------
 // A batch of tensors cut into chunks of kNormChunkBytes; workgroup b sums the chunks [b * perGroup, (b + 1) * perGroup).
-constexpr uint32_t kNormBatch = 240;            // tensors per launch
-constexpr uint32_t kNormGroups = 2048;          // partial sums per launch
+constexpr uint32_t kNormBatch = 240;            // tensors per launch, a multiple of 16
+constexpr uint32_t kNormGroups = 4096;          // partial sums per launch, at most
 constexpr uint32_t kNormChunkBytes = 16384;
 struct NormArgs {
     const void* data[kNormBatch];
-    uint32_t chunkEnd[kNormBatch];      // inclusive prefix of the chunk counts
-    uint32_t lastChunk[kNormBatch];     // elements of the tensor's last chunk, << 2 | type (0 fp32, 1 bf16, 2 fp16)
+    uint32_t chunkEnd[kNormBatch];      // inclusive prefix of the chunk counts, the rest 0xFFFFFFFF
+    uint32_t lastChunk[kNormBatch];     // bytes of the tensor's last chunk, << 2 | type (0 fp32, 1 bf16, 2 fp16)
+    uint32_t groupEnd[16];              // chunkEnd of every sixteenth tensor, the last entry 0xFFFFFFFF
     double* partial;                    // one per workgroup
-    uint32_t nTensors;
     uint32_t nChunks;
     uint32_t perGroup;
 };
-static_assert(sizeof(NormArgs) <= 4096, "kernel arguments");
+static_assert(sizeof(NormArgs) <= 4096 && kNormBatch % 16 == 0 && kNormBatch / 16 < 16, "kernel arguments");
 struct NormJoinArgs {
     const double* partial;
     uint32_t nPartial;
@@ -108,20 +108,13 @@ hipError_t LaunchNormBatch(const NormArgs& args, uint32_t groups, hipStream_t st
 hipError_t LaunchNormJoin(const NormJoinArgs& args, hipStream_t stream);
 
 // ---- AdamW ----------------------------------------------------------------------------------------------------------
-constexpr uint32_t kAdamWBatch = 52;            // tensors per launch
-constexpr uint32_t kAdamWChunk = 4096;          // elements per workgroup, a multiple of the state block
+constexpr uint32_t kAdamWChunk = 2048;          // elements per workgroup, a multiple of the state block
+constexpr uint32_t kAdamWWords = 496;           // words of a launch's table
+// Words of one tensor: its last chunk's inclusive prefix with that chunk's elements in the upper half, param, grad, m, v, then
+// master and the two scales where there are any.
+constexpr uint32_t AdamWTensorWords(bool master, bool fp8State) { return 5u + (master ? 1u : 0u) + (fp8State ? 2u : 0u); }
 struct AdamWArgs {
-    struct Tensor {
-        void* param;
-        const void* grad;
-        void* m;
-        void* v;
-        float* master;
-        float* mScale;
-        float* vScale;
-        uint64_t count;
-    } t[kAdamWBatch];
-    uint32_t chunkEnd[kAdamWBatch];     // inclusive prefix of the chunk counts
+    uint64_t table[kAdamWWords];
     uint32_t nTensors;
     uint32_t skipNonFinite;
     const float* clip;

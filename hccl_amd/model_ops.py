@@ -90,11 +90,10 @@ def _bind(L):
 
 def _address(buf):
     """_as_ptr as a structure's field takes it."""
-    if buf is None or isinstance(buf, int):
-        return buf
-    if hasattr(buf, "data_ptr"):
+    try:
         return buf.data_ptr()
-    return _as_ptr(buf).value
+    except AttributeError:
+        return buf if buf is None or isinstance(buf, int) else _as_ptr(buf).value
 
 
 def token_log_probs_workspace(token_count, vocab_size, top_count=0):
