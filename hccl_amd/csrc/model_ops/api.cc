@@ -90,8 +90,24 @@ HcclResult CheckAligned(const char* name, const void* p, uint64_t to, const char
     return HCCL_SUCCESS;
 }
 
+// Runs the body of an entry point, or of a launch in the rendezvous: no exception leaves through the C boundary, nor past
+// the state of a launch in progress.
+template <class F>
+HcclResult Guarded(const char* name, F body)
+{
+    try {
+        return body();
+    } catch (const std::bad_alloc&) {
+        Log(1, "%s: out of host memory", name);
+        return HCCL_E_MEMORY;
+    } catch (...) {
+        Log(1, "%s: internal error", name);
+        return HCCL_E_INTERNAL;
+    }
+}
+
 // ---- what the last arrival launches -----------------------------------------------------------------------------
-HcclResult RunTokenLogProbs(World* w, PendingOp& p, hipStream_t s)
+HcclResult LaunchTokenLogProbs(World* w, PendingOp& p, hipStream_t s)
 {
     LogProbsArgs a = {};
     const uint64_t rows = p.count;
@@ -175,7 +191,7 @@ uint64_t NormWorkspace(uint64_t tensors)
     return launches * kNormGroups * sizeof(double);
 }
 
-HcclResult RunGradNorm(World* w, PendingOp& p, hipStream_t s)
+HcclResult LaunchGradNorm(World* w, PendingOp& p, hipStream_t s)
 {
     NormJoinArgs join = {};
     uint64_t tensors = 0;
@@ -256,19 +272,14 @@ HcclResult RunGradNorm(World* w, PendingOp& p, hipStream_t s)
     return HCCL_SUCCESS;
 }
 
-// Runs an entry point's body; no exception leaves through the C boundary.
-template <class F>
-HcclResult Guarded(const char* name, F body)
+HcclResult RunTokenLogProbs(World* w, PendingOp& p, hipStream_t s)
 {
-    try {
-        return body();
-    } catch (const std::bad_alloc&) {
-        Log(1, "%s: out of host memory", name);
-        return HCCL_E_MEMORY;
-    } catch (...) {
-        Log(1, "%s: internal error", name);
-        return HCCL_E_INTERNAL;
-    }
+    return Guarded("HcclAmdTokenLogProbs", [&] { return LaunchTokenLogProbs(w, p, s); });
+}
+
+HcclResult RunGradNorm(World* w, PendingOp& p, hipStream_t s)
+{
+    return Guarded("HcclAmdGradNorm", [&] { return LaunchGradNorm(w, p, s); });
 }
 
 // The first checks of every entry point; `ref` is looked up before, so that a collective's call that fails a check keeps

@@ -6,7 +6,7 @@
 // over: d = m - m', s' = s 2^d, t' = 2^d (t + s d).  Then
 //   lse = ln 2 (m + log2 s), log p = ln 2 (y - log2 s), entropy = ln 2 (log2 s - t / s),
 // in which the rounding of m cancels.  That holds while |m| stays small against 2^24; a row whose largest logit lies beyond
-// (lowest values as masks, infinities) is read once more with y = c (x - largest), where nothing but the difference is
+// (lowest values as masks, +inf) is read once more with y = c (x - largest), where nothing but the difference is
 // scaled.
 //
 // Alternatives without a second pass over the row: a histogram of the lane maxima, by their distance from the largest,
@@ -275,6 +275,22 @@ __device__ __forceinline__ uint32_t BlockCount(uint32_t v, TopSpace<kThreads>& s
     return sum;
 }
 
+template <uint32_t kThreads>
+__device__ __forceinline__ uint32_t BlockMax(uint32_t v, TopSpace<kThreads>& sh, uint32_t tid)
+{
+    v = LaneMax(v);
+    __syncthreads();
+    if ((tid & (kWave - 1)) == 0) {
+        sh.waveCount[tid / kWave] = v;
+    }
+    __syncthreads();
+    uint32_t most = 0;
+    for (uint32_t w = 0; w < kThreads / kWave; ++w) {
+        most = sh.waveCount[w] > most ? sh.waveCount[w] : most;
+    }
+    return most;
+}
+
 // Elements of the workgroup's part of the row whose order is at least `bound`.
 template <typename T, uint32_t kThreads>
 __device__ __forceinline__ uint32_t CountFrom(const LogProbsArgs& a, uint64_t row, uint32_t from, uint32_t to, uint32_t bound,
@@ -385,12 +401,13 @@ __device__ __forceinline__ uint32_t SearchTop(const LogProbsArgs& a, uint64_t ro
 }
 
 // A value that `want` lanes reach, or 0 if there are fewer lanes with an element: the lower edge of the first bin of the
-// histogram, counted from the largest value on, up to which `want` lane maxima fall; `reaching` counts them.  Bins are
+// histogram, counted from the largest value on, up to which `want` lane maxima fall; `reaching` counts them and `upper` is
+// the bin's upper edge, where the want-th of them lies at most.  Bins are
 // 2^shift orders wide, first as fine as bfloat16, and wider where the first 255 do not reach far enough.  Every wavefront
 // reads the histogram for itself.
 template <uint32_t kThreads>
 __device__ __forceinline__ uint32_t TopBound(uint32_t laneMost, uint32_t largest, uint32_t want, uint32_t& reaching,
-                                             TopSpace<kThreads>& sh, uint32_t tid)
+                                             uint32_t& upper, TopSpace<kThreads>& sh, uint32_t tid)
 {
     const uint32_t lane = tid & (kWave - 1);
     for (uint32_t shift = 16;; shift += 4) {
@@ -408,6 +425,7 @@ __device__ __forceinline__ uint32_t TopBound(uint32_t laneMost, uint32_t largest
         const uint64_t reached = __ballot(upTo >= want);
         if (reached == 0) {
             reaching = __builtin_amdgcn_readlane(upTo, kWave - 1);
+            upper = largest;
             return 0;
         }
         const uint32_t at = __ffsll(static_cast<unsigned long long>(reached)) - 1;
@@ -420,6 +438,7 @@ __device__ __forceinline__ uint32_t TopBound(uint32_t laneMost, uint32_t largest
         if (bin < kBins - 1 || shift >= 24) {
             // the bin holds orders in (largest - ((bin + 1) << shift), largest - (bin << shift)]
             const uint64_t depth = ((static_cast<uint64_t>(bin) + 1) << shift) - 1;
+            upper = largest - (bin << shift);
             return depth < largest ? largest - static_cast<uint32_t>(depth) : 1u;
         }
         __syncthreads();
@@ -455,10 +474,10 @@ __device__ __forceinline__ bool ListElements(const LogProbsArgs& a, uint64_t row
         return false;
     }
     const float least = bound <= Ordered(-__builtin_inff()) ? -__builtin_inff() : FromOrdered(bound);
-    const uint32_t fetches = 1u << a.slotShift;
-    for (uint32_t item = tid; item < nGroups * (fetches * kUnroll); item += kThreads) {
-        const uint32_t group = sh.group[item / (fetches * kUnroll)];
-        const uint32_t fetch = (group >> 16) * fetches + item / kUnroll % fetches;
+    const uint32_t shift = a.slotShift;
+    for (uint32_t item = tid; item < (nGroups * kUnroll) << shift; item += kThreads) {
+        const uint32_t group = sh.group[(item / kUnroll) >> shift];
+        const uint32_t fetch = ((group >> 16) << shift) + (item / kUnroll & ((1u << shift) - 1u));
         uint32_t begin = 0, start = 0, before = 0;
         uint32_t v = 0, last = 0, count = 0, index = 0;
         const typename T::Raw* data = nullptr;
@@ -504,19 +523,25 @@ __device__ __forceinline__ void GatherTop(const LogProbsArgs& a, uint64_t row, u
                                           uint32_t largest, uint32_t nSlots, const uint16_t* groupMost, TopSpace<kThreads>& sh,
                                           uint32_t tid)
 {
-    uint32_t reaching;
-    const uint32_t bound = TopBound<kThreads>(laneMost, largest, a.topCount, reaching, sh, tid);
+    uint32_t reaching, upper;
+    const uint32_t bound = TopBound<kThreads>(laneMost, largest, a.topCount, reaching, upper, sh, tid);
     // (with fewer lanes than topCount, or a list that a few lanes more than fill, there is nothing to be gained from trying)
     const bool few = reaching <= kCandidates<kThreads> / 4 &&
                      ListElements<T, kThreads>(a, row, from, to, laneMost, bound, nSlots, groupMost, sh, tid);
     if (!few) {
-        uint32_t low = bound, high = largest;      // the exact topCount-th lane maximum
-        while (low < high && reaching >= a.topCount) {
-            const uint32_t mid = low + (high - low + 1) / 2;
-            if (BlockCount<kThreads>(laneMost >= mid ? 1 : 0, sh, tid) >= a.topCount) {
-                low = mid;
-            } else {
-                high = mid - 1;
+        // The exact topCount-th lane maximum: mostly the largest of its bin, else by bisection.
+        uint32_t low = bound;
+        if (reaching >= a.topCount) {
+            uint32_t high = BlockMax<kThreads>(laneMost <= upper ? laneMost : 0u, sh, tid);
+            bool first = true;
+            while (low < high) {
+                const uint32_t mid = first ? high : low + (high - low + 1) / 2;
+                first = false;
+                if (BlockCount<kThreads>(laneMost >= mid ? 1 : 0, sh, tid) >= a.topCount) {
+                    low = mid;
+                } else {
+                    high = mid - 1;
+                }
             }
         }
         __syncthreads();
@@ -719,7 +744,8 @@ __global__ __launch_bounds__(kThreads, kThreads > 256 ? 4 : kTop ? 7 : 8) void L
     uint32_t nSlots;
     Stats all = Pass<T, kThreads, kTop, false>(a, row, from, to, waveStats[0], waveMost, largest, any, groupMost, nSlots, token);
     const float most = LaneMax(lane < kWaves ? waveMost[lane] : -__builtin_inff());     // of the workgroup
-    const bool safe = !(fabsf(most * a.exp2Scale) <= kReach);
+    // (-inf alone leaves s = 0, or a NaN, in either form)
+    const bool safe = most != -__builtin_inff() && !(fabsf(most * a.exp2Scale) <= kReach);
     if (safe) {
         __syncthreads();      // (the maxima above are overwritten)
         all = Pass<T, kThreads, kTop, true>(a, row, from, to, waveStats[1], waveMost, largest, any, groupMost, nSlots, token);

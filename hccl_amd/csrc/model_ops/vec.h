@@ -179,22 +179,18 @@ __device__ __forceinline__ double XorLane(double v)
     return __builtin_bit_cast(double, U32x2{XorLane<D>(w.x), XorLane<D>(w.y)});
 }
 
-// Reductions over groups of kLanes neighbouring lanes; every lane gets the result, and all the same bits (the operands of
-// a pair only change places).
-template <uint32_t kLanes = kWave>
-__device__ __forceinline__ float LaneMax(float v)
+// Reductions over a wavefront; every lane gets the result, and all the same bits (the operands of a pair only change places).
+__device__ __forceinline__ float Larger(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ uint32_t Larger(uint32_t a, uint32_t b) { return a > b ? a : b; }
+template <typename V>
+__device__ __forceinline__ V LaneMax(V v)
 {
-    v = fmaxf(v, XorLane<1>(v));
-    v = fmaxf(v, XorLane<2>(v));
-    v = fmaxf(v, XorLane<4>(v));
-    v = fmaxf(v, XorLane<8>(v));
-    if constexpr (kLanes >= 32) {
-        v = fmaxf(v, XorLane<16>(v));
-    }
-    if constexpr (kLanes >= 64) {
-        v = fmaxf(v, XorLane<32>(v));
-    }
-    return v;
+    v = Larger(v, XorLane<1>(v));
+    v = Larger(v, XorLane<2>(v));
+    v = Larger(v, XorLane<4>(v));
+    v = Larger(v, XorLane<8>(v));
+    v = Larger(v, XorLane<16>(v));
+    return Larger(v, XorLane<32>(v));
 }
 template <typename V>
 __device__ __forceinline__ V WaveSum(V v)

@@ -13,6 +13,7 @@ one thread inside ``with hccl_amd.group():``.  What the arguments mean is writte
 """
 import ctypes
 import os
+import struct
 
 import hccl_amd
 from hccl_amd import HcclDataType, _as_ptr, _as_stream, check
@@ -59,6 +60,22 @@ class AdamWConfig(ctypes.Structure):
                 ("stepOnDevice", _vp), ("lrOnDevice", _vp), ("clip", _vp), ("stateType", _i32), ("skipNonFinite", _i32)]
 
 
+def _packer(cls):
+    """Packs the fields of the structure `cls`, in order, into the bytes an entry point reads: a fifth of the time the
+    ctypes structure itself takes, which counts in calls of a few microseconds."""
+    code = {_vp: "Q", _u64: "Q", _u32: "I", _i32: "i", _f32: "f", _f64: "d"}
+    packer = struct.Struct("@" + "".join(code[t] for _, t in cls._fields_) + "0Q")
+    assert packer.size == ctypes.sizeof(cls)
+    return packer.pack
+
+
+_pack_log_probs = _packer(TokenLogProbsArgs)
+_pack_grad = _packer(TokenLogProbsGradArgs)
+_pack_config = _packer(AdamWConfig)
+_pack_norm = _packer(NormTensor)
+_pack_adamw = _packer(AdamWTensor)
+_ADAMW_FIELDS = frozenset(("param", "grad", "exp_avg", "exp_avg_sq", "master", "exp_avg_scale", "exp_avg_sq_scale", "count",
+                           "param_type", "grad_type"))
 _lib = None
 
 
@@ -76,12 +93,12 @@ def lib():
 
 def _bind(L):
     """Declares the argument and result types of the library's entry points on the loaded library L."""
-    L.HcclAmdTokenLogProbs.argtypes = [ctypes.POINTER(TokenLogProbsArgs), _vp, _vp]
+    L.HcclAmdTokenLogProbs.argtypes = [_vp, _vp, _vp]
     L.HcclAmdTokenLogProbsWorkspace.argtypes = [_u64, _u64, _u32, ctypes.POINTER(_u64)]
-    L.HcclAmdTokenLogProbsGrad.argtypes = [ctypes.POINTER(TokenLogProbsGradArgs), _vp, _vp]
+    L.HcclAmdTokenLogProbsGrad.argtypes = [_vp, _vp, _vp]
     L.HcclAmdGradNorm.argtypes = [ctypes.POINTER(NormTensor), _u32, _f32, _f32, _vp, _vp, _u64, _vp, _vp]
     L.HcclAmdGradNormWorkspace.argtypes = [_u64, ctypes.POINTER(_u64)]
-    L.HcclAmdAdamW.argtypes = [ctypes.POINTER(AdamWTensor), _u32, ctypes.POINTER(AdamWConfig), _vp, _vp]
+    L.HcclAmdAdamW.argtypes = [ctypes.POINTER(AdamWTensor), _u32, _vp, _vp, _vp]
     for name in ("HcclAmdTokenLogProbs", "HcclAmdTokenLogProbsWorkspace", "HcclAmdTokenLogProbsGrad", "HcclAmdGradNorm",
                  "HcclAmdGradNormWorkspace", "HcclAmdAdamW"):
         getattr(L, name).restype = ctypes.c_int
@@ -89,11 +106,13 @@ def _bind(L):
 
 
 def _address(buf):
-    """_as_ptr as a structure's field takes it."""
+    """_as_ptr as a number; 0 for None."""
+    if buf is None:
+        return 0
     try:
         return buf.data_ptr()
     except AttributeError:
-        return buf if buf is None or isinstance(buf, int) else _as_ptr(buf).value
+        return buf if isinstance(buf, int) else _as_ptr(buf).value or 0
 
 
 def token_log_probs_workspace(token_count, vocab_size, top_count=0):
@@ -105,36 +124,36 @@ def token_log_probs_workspace(token_count, vocab_size, top_count=0):
 
 
 def token_log_probs(hccl_comm, logits, token_count, vocab_start, vocab_count, tokens, log_probs,
-                    data_type=HcclDataType.BFP16, token_type=HcclDataType.INT64, row_stride=None, scale=1.0, lse=None,
+                    data_type=HcclDataType.FP32, token_type=HcclDataType.INT64, row_stride=None, scale=1.0, lse=None,
                     entropy=None, top_count=0, top_values=None, top_ids=None, workspace=None, workspace_bytes=0,
                     stream=None):
     """Log probabilities of `tokens` under softmax(scale * logits), whose columns vocab_start .. vocab_start + vocab_count
     this rank holds; every output (log_probs, lse, entropy, top_values, top_ids) may be None."""
-    args = TokenLogProbsArgs(_address(logits), vocab_count if row_stride is None else row_stride, vocab_start, vocab_count,
-                             token_count, _address(tokens), data_type, token_type, scale, top_count, _address(log_probs),
-                             _address(lse), _address(entropy), _address(top_values), _address(top_ids),
-                             _address(workspace), workspace_bytes)
+    args = _pack_log_probs(_address(logits), vocab_count if row_stride is None else row_stride, vocab_start, vocab_count,
+                           token_count, _address(tokens), data_type, token_type, scale, top_count, _address(log_probs),
+                           _address(lse), _address(entropy), _address(top_values), _address(top_ids),
+                           _address(workspace), workspace_bytes)
     return check(lib().HcclAmdTokenLogProbs(args, hccl_comm, _as_stream(stream)), "HcclAmdTokenLogProbs")
 
 
 def token_log_probs_grad(hccl_comm, logits, token_count, vocab_start, vocab_count, tokens, lse, grad_log_probs, grad_logits,
-                         data_type=HcclDataType.BFP16, token_type=HcclDataType.INT64, row_stride=None,
+                         data_type=HcclDataType.FP32, token_type=HcclDataType.INT64, row_stride=None,
                          grad_row_stride=None, scale=1.0, entropy=None, grad_entropy=None, top_count=0, top_ids=None,
                          grad_top_values=None, stream=None):
     """Writes the gradient with respect to this rank's part of the logits to `grad_logits` (which may be the logits
     themselves); local to the rank."""
-    args = TokenLogProbsGradArgs(_address(logits), vocab_count if row_stride is None else row_stride, vocab_start,
-                                 vocab_count, token_count, _address(tokens), data_type, token_type, scale, top_count,
-                                 _address(lse), _address(entropy), _address(grad_log_probs), _address(grad_entropy),
-                                 _address(top_ids), _address(grad_top_values), _address(grad_logits),
-                                 vocab_count if grad_row_stride is None else grad_row_stride)
+    args = _pack_grad(_address(logits), vocab_count if row_stride is None else row_stride, vocab_start, vocab_count,
+                      token_count, _address(tokens), data_type, token_type, scale, top_count, _address(lse),
+                      _address(entropy), _address(grad_log_probs), _address(grad_entropy), _address(top_ids),
+                      _address(grad_top_values), _address(grad_logits),
+                      vocab_count if grad_row_stride is None else grad_row_stride)
     return check(lib().HcclAmdTokenLogProbsGrad(args, hccl_comm, _as_stream(stream)), "HcclAmdTokenLogProbsGrad")
 
 
 def norm_tensors(tensors):
     """The array grad_norm takes, from (buffer, count, data type) triples; it can be kept while the buffers stay."""
-    items = [NormTensor(_address(buf), count, int(data_type)) for buf, count, data_type in tensors]
-    return (NormTensor * len(items))(*items)
+    items = [_pack_norm(_address(buf), count, data_type) for buf, count, data_type in tensors]
+    return (NormTensor * len(items)).from_buffer_copy(b"".join(items))
 
 
 def grad_norm_workspace(tensor_count):
@@ -158,15 +177,12 @@ def adamw_tensors(tensors):
     they are wanted, master, exp_avg_scale, exp_avg_sq_scale; it can be kept while the buffers stay."""
     items = []
     for t in tensors:
-        unknown = set(t) - {"param", "grad", "exp_avg", "exp_avg_sq", "master", "exp_avg_scale", "exp_avg_sq_scale",
-                            "count", "param_type", "grad_type"}
-        if unknown:
-            raise TypeError("adamw_tensors: unknown fields %s" % sorted(unknown))
-        items.append(AdamWTensor(_address(t["param"]), _address(t["grad"]), _address(t["exp_avg"]),
-                                 _address(t["exp_avg_sq"]), _address(t.get("master")), _address(t.get("exp_avg_scale")),
-                                 _address(t.get("exp_avg_sq_scale")), t["count"], int(t["param_type"]),
-                                 int(t["grad_type"])))
-    return (AdamWTensor * len(items))(*items)
+        if not _ADAMW_FIELDS.issuperset(t):
+            raise TypeError("adamw_tensors: unknown fields %s" % sorted(set(t) - _ADAMW_FIELDS))
+        items.append(_pack_adamw(_address(t["param"]), _address(t["grad"]), _address(t["exp_avg"]), _address(t["exp_avg_sq"]),
+                                 _address(t.get("master")), _address(t.get("exp_avg_scale")),
+                                 _address(t.get("exp_avg_sq_scale")), t["count"], t["param_type"], t["grad_type"]))
+    return (AdamWTensor * len(items)).from_buffer_copy(b"".join(items))
 
 
 def adamw(hccl_comm, tensors, step, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01,
@@ -176,6 +192,6 @@ def adamw(hccl_comm, tensors, step, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight
     grad_norm result; `step` counts from 1 (step_on_device: an int64 on the device that is read instead)."""
     if not isinstance(tensors, ctypes.Array):
         tensors = adamw_tensors(tensors)
-    config = AdamWConfig(lr, beta1, beta2, eps, weight_decay, step, _address(step_on_device), _address(lr_on_device),
-                         _address(clip), int(state_type), 1 if skip_non_finite else 0)
+    config = _pack_config(lr, beta1, beta2, eps, weight_decay, step, _address(step_on_device), _address(lr_on_device),
+                          _address(clip), state_type, 1 if skip_non_finite else 0)
     return check(lib().HcclAmdAdamW(tensors, len(tensors), config, hccl_comm, _as_stream(stream)), "HcclAmdAdamW")

@@ -719,6 +719,67 @@ def test_adamw_quantises_as_the_type_says(worlds):
     assert torch.equal(got["exp_avg"][clean], want[clean])
 
 
+# ---- beyond 32 bits -----------------------------------------------------------------------------------------------------
+def test_logits_beyond_32_bits_of_elements(worlds):
+    """2^32 logits and a few rows more, in place: the last rows lie beyond every 32-bit offset."""
+    v, t = 131072, (1 << 15) + 5
+    w = worlds(1)
+    x = torch.zeros(t, v, dtype=torch.bfloat16, device="cuda")
+    tail = (rng_tensor(3, 6, v) * 2).to(torch.bfloat16)
+    x[-6:] = tail.cuda()
+    tokens = torch.full((t,), 11, device="cuda")
+    tokens[:-6] = -100
+    lp, lse, ent = (torch.full((t,), FILL, device="cuda") for _ in range(3))
+    ids = torch.zeros(t, 3, dtype=torch.int64, device="cuda")
+    values = torch.zeros(t, 3, device="cuda")
+    g = torch.full((t,), 0.5, device="cuda")
+    torch.cuda.synchronize()
+    model_ops.token_log_probs(w.comms[0], x, t, 0, v, tokens, lp, data_type=DT.BFP16, lse=lse, entropy=ent, top_count=3, top_values=values,
+                              top_ids=ids, stream=w.stream)
+    model_ops.token_log_probs_grad(w.comms[0], x, t, 0, v, tokens, lse, g, x, data_type=DT.BFP16, entropy=ent,
+                                   grad_entropy=g, stream=w.stream)
+    w.sync()
+    rows = Rows(tail, DT.BFP16, 1, 3, parts=[(0, v)])
+    got = tuple(a[-6:].cpu().double() for a in (lp, lse, ent, values)) + (ids[-6:].cpu(),)
+    eleven = torch.full((6,), 11)
+    check_rows(rows, got, eleven, 1.0)
+    check_grad(rows, x[-6:].cpu(), got[1], got[2], None, eleven, 1.0, g[-6:].cpu(), g[-6:].cpu(), None)
+    # rows of zeros: uniform, whose entropy has no gradient beyond rounding
+    assert abs(float(lse[7]) - math.log(v)) < 1e-5 and lp[7] == 0 and ids[7].tolist() == [0, 1, 2]
+    assert float(x[:8].float().abs().max()) < 1e-9
+
+
+def test_tensors_beyond_32_bits_of_elements(worlds):
+    n, tail = (1 << 32) + 1000, 3000
+    w = worlds(1)
+    param = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    grad = torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    m = torch.zeros(n, dtype=torch.uint8, device="cuda")
+    v = torch.zeros(n, dtype=torch.uint8, device="cuda")
+    m_scale, v_scale = (torch.zeros(-(-n // 256), device="cuda") for _ in range(2))
+    weights, g = (rng_tensor(5, tail, scale=0.1)).to(torch.bfloat16), (rng_tensor(6, tail, scale=0.1)).to(torch.bfloat16)
+    param[-tail:], grad[-tail:] = weights.cuda(), g.cuda()
+    result = torch.zeros(2, device="cuda")
+    space = torch.empty(model_ops.grad_norm_workspace(1), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    model_ops.grad_norm(w.comms[0], [(grad, n, DT.BFP16)], 0.0, result, workspace=space, workspace_bytes=space.numel(),
+                        stream=w.stream)
+    model_ops.adamw(w.comms[0], [dict(param=param, grad=grad, exp_avg=m, exp_avg_sq=v, exp_avg_scale=m_scale,
+                                      exp_avg_sq_scale=v_scale, count=n, param_type=DT.BFP16, grad_type=DT.BFP16)],
+                    1, 1e-2, 0.9, 0.99, 1e-8, 0.1, DT.FP8E4M3, clip=result, stream=w.stream)
+    w.sync()
+    norm = float(g.double().square().sum().sqrt())
+    assert abs(float(result[0]) - norm) <= 2 * U * norm and float(result[1]) == 1.0
+    update = 1e-2 * g.double() / (g.double().abs() + 1e-8)         # the first step's m / sqrt(v) is the gradient's sign
+    want = weights.double() * (1 - 1e-3) - update
+    assert bool(((param[-tail:].cpu().double() - want).abs() <= 2.0 ** -8 * want.abs() + 64 * U * 1e-2).all())
+    last = -(-n // 256) - 1
+    assert float(m_scale[last]) > 0 and float(m_scale[0]) == 0 and not bool(param[:-tail].any())
+    codes = wide(m[last * 256:].cpu(), m_scale[last:].cpu())
+    near = 0.1 * g.double()[-codes.numel():]
+    assert bool(((codes - near).abs() <= torch.maximum(near.abs() * 2.0 ** -4, m_scale[last].cpu().double() * 2.0 ** -10) * 1.001).all())
+
+
 # ---- together ---------------------------------------------------------------------------------------------------------
 def test_calls_can_be_captured_into_a_graph_and_replayed(worlds):
     """The log probabilities in both forms (rows that share workgroups and rows that do not), their gradient, the norm and
@@ -796,6 +857,60 @@ def test_calls_can_be_captured_into_a_graph_and_replayed(worlds):
         count += 1
         few_tokens.add_(1)
         torch.cuda.synchronize()
+
+
+def test_blocking_calls_from_one_thread_per_rank(worlds):
+    """Every rank's thread, on a stream of its own, alternates these collectives with the data plane's and local steps."""
+    import threading
+    n, t, v = 3, 5, 3001
+    w = World(n)
+    try:
+        x = rng_tensor(1, t, v)
+        rows = Rows(x, DT.FP32, n, 4)
+        tokens = given(t, v, 1)
+        want = rows.run(w, tokens)
+        dev = tokens.cuda()
+        streams = [torch.cuda.Stream() for _ in range(n)]
+        sums = [torch.zeros(100, device="cuda") for _ in range(n)]
+        ones = torch.ones(100, device="cuda")
+        results = torch.zeros(n, 2, device="cuda")
+        spaces = [torch.empty(1 << 20, dtype=torch.uint8, device="cuda") for _ in range(n)]
+        states = [[torch.zeros(100, device="cuda") for _ in range(3)] for _ in range(n)]
+        errors = []
+        torch.cuda.synchronize()
+
+        def rank(r):
+            try:
+                start, count = rows.parts[r]
+                s = rows.shards[r]
+                for step in range(1, 13):
+                    model_ops.token_log_probs(w.comms[r], s if count else None, t, start, count, dev, rows.log_probs[r],
+                                              data_type=DT.FP32, row_stride=s.stride(0), lse=rows.lse[r],
+                                              entropy=rows.entropy[r], top_count=4, top_values=rows.values[r],
+                                              top_ids=rows.ids[r], workspace=spaces[r], workspace_bytes=1 << 20,
+                                              stream=streams[r])
+                    hccl_amd.all_reduce(w.comms[r], ones, sums[r], 100, DT.FP32, OP.SUM, streams[r])
+                    model_ops.grad_norm(w.comms[r], [(sums[r], 100, DT.FP32)], 1.0, results[r], workspace=spaces[r],
+                                        workspace_bytes=1 << 20, stream=streams[r])
+                    model_ops.adamw(w.comms[r], [dict(param=states[r][0], grad=sums[r], exp_avg=states[r][1],
+                                                      exp_avg_sq=states[r][2], count=100, param_type=DT.FP32,
+                                                      grad_type=DT.FP32)], step, 0.1, clip=results[r], stream=streams[r])
+            except Exception as e:      # a thread's failure must not look like success
+                errors.append(e)
+        threads = [threading.Thread(target=rank, args=(r,)) for r in range(n)]
+        for th in threads:
+            th.start()
+        for th in threads:
+            th.join(60)
+        torch.cuda.synchronize()
+        assert not errors, errors
+        assert torch.equal(rows.log_probs[0][:-1].cpu().double().nan_to_num(9e9), want[0].nan_to_num(9e9))
+        norm = math.sqrt(100 * n * n * n)
+        assert abs(float(results[1, 0]) - norm) <= 2 * U * norm and torch.equal(results, results[:1].expand(n, 2))
+        assert torch.equal(states[0][0], states[1][0]) and torch.equal(states[0][0], states[2][0])
+        assert float(states[0][0].max()) < -1.0           # a dozen steps of about 0.1 against a constant gradient
+    finally:
+        w.close()
 
 
 def test_a_sharded_training_step(worlds):
