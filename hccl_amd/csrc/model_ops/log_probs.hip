@@ -148,7 +148,7 @@ struct Part {
     __device__ __forceinline__ uint32_t Base(uint32_t v) const { return v < full ? v * P : count >= P ? count - P : 0u; }
     __device__ __forceinline__ U32x4 Load(uint32_t v) const
     {
-        if (v < full) {
+        if (__builtin_expect(v < full, 1)) {
             return LoadOnce16(row + static_cast<uint64_t>(v) * P);
         }
         U32x4 raw = {kNone, kNone, kNone, kNone};
@@ -435,7 +435,7 @@ __device__ __forceinline__ uint32_t TopBound(uint32_t laneMost, uint32_t largest
             reaching += __builtin_amdgcn_readlane(n[i], at);
             bin += reaching < want ? 1 : 0;
         }
-        if (bin < kBins - 1 || shift >= 24) {
+        if (__builtin_expect(bin < kBins - 1 || shift >= 24, 1)) {
             // the bin holds orders in (largest - ((bin + 1) << shift), largest - (bin << shift)]
             const uint64_t depth = ((static_cast<uint64_t>(bin) + 1) << shift) - 1;
             upper = largest - (bin << shift);
@@ -528,7 +528,7 @@ __device__ __forceinline__ void GatherTop(const LogProbsArgs& a, uint64_t row, u
     // (with fewer lanes than topCount, or a list that a few lanes more than fill, there is nothing to be gained from trying)
     const bool few = reaching <= kCandidates<kThreads> / 4 &&
                      ListElements<T, kThreads>(a, row, from, to, laneMost, bound, nSlots, groupMost, sh, tid);
-    if (!few) {
+    if (__builtin_expect(!few, 0)) {
         // The exact topCount-th lane maximum: mostly the largest of its bin, else by bisection.
         uint32_t low = bound;
         if (reaching >= a.topCount) {
@@ -746,7 +746,7 @@ __global__ __launch_bounds__(kThreads, kThreads > 256 ? 4 : kTop ? 7 : 8) void L
     const float most = LaneMax(lane < kWaves ? waveMost[lane] : -__builtin_inff());     // of the workgroup
     // (-inf alone leaves s = 0, or a NaN, in either form)
     const bool safe = most != -__builtin_inff() && !(fabsf(most * a.exp2Scale) <= kReach);
-    if (safe) {
+    if (__builtin_expect(safe, 0)) {
         __syncthreads();      // (the maxima above are overwritten)
         all = Pass<T, kThreads, kTop, true>(a, row, from, to, waveStats[1], waveMost, largest, any, groupMost, nSlots, token);
     }
