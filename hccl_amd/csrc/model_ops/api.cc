@@ -25,7 +25,7 @@ bool Aligned(const void* p, uint64_t to) { return (reinterpret_cast<uintptr_t>(p
 
 constexpr uint64_t kMaxVocab = 0x7FFFFFFFull;
 constexpr uint64_t kMaxRows = (1ull << 24) - 1;
-constexpr uint64_t kMaxRowStride = 1ull << 40;      // rows x stride x 4 bytes stays far below 2^64
+constexpr uint64_t kMaxRowStride = 1ull << 36;      // rows x stride x 4 bytes stays below 2^62
 
 // A structure of a rank's call as the words RankArgs::var carries, and back.
 template <typename S>
@@ -164,8 +164,8 @@ HcclResult LaunchTokenLogProbs(World* w, PendingOp& p, hipStream_t s)
                 (unsigned long long)vocab, (unsigned long long)need);
             return HCCL_E_MEMORY;
         }
-        a.stats = static_cast<float*>(space);
-        a.keys = reinterpret_cast<uint64_t*>(a.stats + rows * a.nSplit * 4);
+        a.stats = static_cast<LogProbsStats*>(space);
+        a.keys = reinterpret_cast<uint64_t*>(a.stats + rows * a.nSplit);
     }
     HIP_OK(LaunchLogProbs(a, p.dtype, static_cast<uint32_t>(rows), s));
     return HCCL_SUCCESS;

@@ -1,13 +1,15 @@
 // Log probabilities of given tokens, entropy and top alternatives of rows of logits whose vocabulary lies in up to 64
 // parts (one per rank).
 //
-// One pass over a row keeps, per lane, the largest logit, a reference m = c * largest (c = scale * log2 e, no lower than
-// -2^20), s = sum exp2(y) and t = sum y exp2(y) with y = c x - m in one multiply-add.  Whenever m grows, both are carried
-// over: d = m - m', s' = s 2^d, t' = 2^d (t + s d).  Then
-//   lse = ln 2 (m + log2 s), log p = ln 2 (y - log2 s), entropy = ln 2 (log2 s - t / s),
-// in which the rounding of m cancels.  That holds while |m| stays small against 2^24; a row whose largest logit lies beyond
-// (lowest values as masks, +inf) is read once more with y = c (x - largest), where nothing but the difference is
-// scaled.
+// One pass over a row keeps, per lane, the largest logit m, s = sum exp2(y) and t = sum y exp2(y) with y = c (x - m),
+// c = scale * log2 e.  Whenever m grows, both are carried over: d = c (m - m'), s' = s 2^d, t' = 2^d (t + s d).  Then
+//   lse = scale m + ln s, log p = scale (x - m) - ln s, entropy = ln s - ln 2 t / s.
+// The difference is formed before it is scaled: the largest logit's y is exactly 0, so that a probability near 1 keeps its
+// digits, and rows of the type's lowest value (a mask) come out like any other row of equal logits.  (c x - m' in one
+// multiply-add saves an instruction per element, not measurably any time, and loses both.)  s is 64 bits wide: eight terms
+// are added in 32 bits in three roundings, everything else in 64, and ln s takes the digits that 32 bits lack.  With a
+// likely token, ln s near 0, the error of log p is then 1.8e-6 of it at any row length (1.3e-5 at 32768 entries with s in
+// 32 bits, which is 0.5 % faster; 4.9e-6 as torch adds).
 //
 // Alternatives without a second pass over the row: a histogram of the lane maxima, by their distance from the largest,
 // yields a bound that topCount lanes reach, and so topCount elements.  Every lane also leaves the largest of each group of
@@ -35,7 +37,6 @@ constexpr uint32_t kGroupBytes = 16384;    // LDS for the groups' maxima, at mos
 constexpr float kLowest = -3.402823466e38f;
 constexpr float kFarBelow = -1e30f;        // stands for -inf where it is multiplied by a zero probability
 constexpr float kLn2 = 0.69314718055994531f;
-constexpr float kReach = 1048576.0f;       // largest reference whose rounding is harmless
 
 // Order of floats as unsigned integers; both zeros are one value.
 __device__ __forceinline__ uint32_t Ordered(float x)
@@ -53,56 +54,48 @@ __device__ __forceinline__ uint64_t Key(uint32_t ordered, uint32_t index)
     return (static_cast<uint64_t>(ordered) << 32) | (0xFFFFFFFFu - index);
 }
 
-// Sums of a set of elements relative to a reference: kSafe: the largest logit itself, otherwise c * that.
-struct Stats {
-    float m, s, t;
-};
+typedef LogProbsStats Stats;
+constexpr Stats kNoElements = {kLowest, 0.0f, 0.0};      // (or -inf alone)
 
-template <bool kSafe>
 __device__ __forceinline__ void Rescale(Stats& a, float m, float c)
 {
-    const float d = kSafe ? fmaxf((a.m - m) * c, kFarBelow) : a.m - m;
+    const float d = fmaxf((a.m - m) * c, kFarBelow);
     const float f = Exp2(d);
-    a.t = f * __builtin_fmaf(a.s, d, a.t);
-    a.s = a.s * f;
+    a.t = f * __builtin_fmaf(static_cast<float>(a.s), d, a.t);
+    a.s = a.s * static_cast<double>(f);
     a.m = m;
 }
 
 // The same for a wavefront's sets together.
-template <bool kSafe>
 __device__ __forceinline__ Stats WaveJoin(Stats a, float c)
 {
     Stats r;
     r.m = LaneMax(a.m);
-    Rescale<kSafe>(a, r.m, c);
+    Rescale(a, r.m, c);
     r.s = WaveSum(a.s);
     r.t = WaveSum(a.t);
     return r;
 }
 
-template <bool kSafe>
-__device__ __forceinline__ Stats NoElements()
-{
-    return Stats{kSafe ? kLowest : -kReach, 0.0f, 0.0f};
-}
-
-// N more elements, of which the largest is returned; `largest` is the lane's largest logit so far.
-template <bool kSafe, uint32_t N>
-__device__ __forceinline__ float Accumulate(Stats& a, float& largest, const float* x, float c)
+// N more elements, of which the largest is returned.
+template <uint32_t N>
+__device__ __forceinline__ float Accumulate(Stats& a, const float* x, float c)
 {
     float most = x[0];
     for (uint32_t i = 1; i < N; ++i) {
         most = fmaxf(most, x[i]);
     }
-    if (most > largest) {
-        largest = most;
-        Rescale<kSafe>(a, fmaxf(kSafe ? most : most * c, a.m), c);
+    if (most > a.m) {
+        Rescale(a, most, c);
     }
+    float e[N];
     for (uint32_t i = 0; i < N; ++i) {
-        const float y = kSafe ? (x[i] - a.m) * c : __builtin_fmaf(x[i], c, -a.m);
-        const float e = Exp2(y);
-        a.s += e;
-        a.t = __builtin_fmaf(fmaxf(y, kFarBelow), e, a.t);
+        const float y = (x[i] - a.m) * c;
+        e[i] = Exp2(y);
+        a.t = __builtin_fmaf(fmaxf(y, kFarBelow), e[i], a.t);
+    }
+    for (uint32_t i = 0; i < N; i += 8) {
+        a.s += static_cast<double>(((e[i] + e[i + 1]) + (e[i + 2] + e[i + 3])) + ((e[i + 4] + e[i + 5]) + (e[i + 6] + e[i + 7])));
     }
     return most;
 }
@@ -571,30 +564,27 @@ __device__ __forceinline__ void GatherTop(const LogProbsArgs& a, uint64_t row, u
 
 // What is written for a row once its numbers are known.
 struct RowResult {
-    float m, log2Sum, lse, entropy;
-    bool safe;      // how m is meant, see Stats
+    float m, logSum, lse, entropy;
     bool none;      // -inf alone
     bool bad;       // a NaN or +inf
 };
 
-__device__ __forceinline__ RowResult Finish(Stats a, bool safe, const LogProbsArgs& k)
+__device__ __forceinline__ RowResult Finish(Stats a, float scale)
 {
     RowResult r;
     r.m = a.m;
-    r.safe = safe;
-    r.none = a.s == 0.0f;
-    r.bad = a.s != a.s;
-    r.log2Sum = log2f(a.s);
-    r.lse = r.none ? -__builtin_inff() : safe ? __builtin_fmaf(a.m, k.scale, r.log2Sum * kLn2) : (a.m + r.log2Sum) * kLn2;
-    r.entropy = r.none ? 0.0f : kLn2 * (r.log2Sum - a.t / a.s);
+    const float s = static_cast<float>(a.s);
+    r.none = s == 0.0f;
+    r.bad = s != s;
+    r.logSum = logf(s) + static_cast<float>(a.s - static_cast<double>(s)) / s;      // ln s to all 32 bits also next to s = 1
+    r.lse = r.none ? -__builtin_inff() : __builtin_fmaf(a.m, scale, r.logSum);
+    r.entropy = r.none ? 0.0f : r.logSum - kLn2 * (a.t / s);
     return r;
 }
 
-__device__ __forceinline__ float LogProbOf(const RowResult& r, float x, const LogProbsArgs& k)
+__device__ __forceinline__ float LogProbOf(const RowResult& r, float x, float scale)
 {
-    const float y = r.safe ? (x - r.m) * k.exp2Scale : __builtin_fmaf(x, k.exp2Scale, -r.m);
-    // (far below the others the logit itself decides, and c x may be beyond a float where scale x is not)
-    return r.none ? -__builtin_inff() : y < -kReach ? __builtin_fmaf(x, k.scale, -r.lse) : kLn2 * (y - r.log2Sum);
+    return r.none ? -__builtin_inff() : __builtin_fmaf(x - r.m, scale, -r.logSum);
 }
 
 // The given token of a row and its logit, fetched before the reductions that the result waits for.
@@ -634,11 +624,11 @@ __device__ __forceinline__ void WriteRow(const LogProbsArgs& a, uint64_t row, co
         value = __builtin_nanf("");
         if (!r.bad) {
             const uint64_t key = top[lane];
-            value = LogProbOf(r, FromOrdered(static_cast<uint32_t>(key >> 32)), a);
+            value = LogProbOf(r, FromOrdered(static_cast<uint32_t>(key >> 32)), a.scale);
             id = static_cast<int64_t>(0xFFFFFFFFu - static_cast<uint32_t>(key));
         }
     }
-    const float logProb = token.id >= a.vocab ? __builtin_nanf("") : token.id >= 0 ? LogProbOf(r, token.logit, a) : 0.0f;
+    const float logProb = token.id >= a.vocab ? __builtin_nanf("") : token.id >= 0 ? LogProbOf(r, token.logit, a.scale) : 0.0f;
     for (uint32_t o = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave); o < a.nOut; o += kThreads / kWave) {
         const LogProbsArgs::Out& out = a.out[o];
         if (lane == 0) {
@@ -668,59 +658,13 @@ __device__ __forceinline__ void WriteRow(const LogProbsArgs& a, uint64_t row, co
     }
 }
 
-// One pass over the workgroup's part of the row, joined over the workgroup; `largest` is the lane's largest logit, and with
-// kTop groupMost[slot][lane] the order, cut to 16 bits, of the largest of 2^slotShift fetches.
-template <typename T, uint32_t kThreads, bool kTop, bool kSafe>
-__device__ __forceinline__ Stats Pass(const LogProbsArgs& a, uint64_t row, uint32_t from, uint32_t to, Stats* waveStats,
-                                      float* waveMost, float& largest, bool& any, uint16_t* groupMost, uint32_t& nSlots, Token& token)
-{
-    constexpr uint32_t kWaves = kThreads / kWave;
-    const uint32_t lane = threadIdx.x & (kWave - 1);
-    Stats acc = NoElements<kSafe>();
-    largest = -__builtin_inff();
-    Reader<T, kThreads> reader(a, row, from, to);
-    U32x4 raw[kUnroll];
-    uint32_t fetch = 0, slotMost = 0;
-    while (reader.Fetch(raw)) {
-        float x[kUnroll * kPer16<T>];
-        for (uint32_t u = 0; u < kUnroll; ++u) {
-            Unpack16<T>(raw[u], x + u * kPer16<T>);
-        }
-        if (!kSafe && fetch == 0) {
-            token.logit = TokenLogit<T>(a, row, token.id);      // on its way while the row is read
-        }
-        const float most = Accumulate<kSafe, kUnroll * kPer16<T>>(acc, largest, x, a.exp2Scale);
-        if constexpr (kTop) {
-            const uint32_t order = Ordered(most) >> 16;
-            slotMost = (fetch & ((1u << a.slotShift) - 1u)) != 0 && slotMost > order ? slotMost : order;
-            groupMost[(fetch >> a.slotShift) * kThreads + threadIdx.x] = static_cast<uint16_t>(slotMost);
-        }
-        ++fetch;
-    }
-    nSlots = (fetch + (1u << a.slotShift) - 1) >> a.slotShift;
-    any = reader.any;
-    const Stats wave = WaveJoin<kSafe>(acc, a.exp2Scale);
-    const float most = LaneMax(largest);
-    if (lane == 0) {
-        waveStats[threadIdx.x / kWave] = wave;
-        waveMost[threadIdx.x / kWave] = most;
-    }
-    __syncthreads();
-    Stats all = NoElements<kSafe>();
-    if (lane < kWaves) {
-        all = waveStats[lane];
-    }
-    return WaveJoin<kSafe>(all, a.exp2Scale);
-}
-
 template <typename T, uint32_t kThreads, bool kTop>
 __global__ __launch_bounds__(kThreads, kThreads > 256 ? 4 : kTop ? 7 : 8) void LogProbsKernel(const LogProbsArgs a)
 {
-    constexpr uint32_t kWaves = kThreads / kWave;
-    __shared__ Stats waveStats[2][kWaves];
-    __shared__ float waveMost[kWaves];
+    constexpr uint32_t P = kPer16<T>, kWaves = kThreads / kWave;
+    __shared__ Stats waveStats[kWaves];
     __shared__ TopSpace<kTop ? kThreads : kWave> sh;
-    extern __shared__ uint16_t groupMost[];
+    extern __shared__ uint16_t groupMost[];      // [slot][lane]: order, cut to 16 bits, of the largest of 2^slotShift fetches
     const uint32_t tid = threadIdx.x, lane = tid & (kWave - 1);
     const uint32_t split = blockIdx.x % a.nSplit;
     const uint64_t row = blockIdx.x / a.nSplit;
@@ -739,21 +683,39 @@ __global__ __launch_bounds__(kThreads, kThreads > 256 ? 4 : kTop ? 7 : 8) void L
             sh.nCandidates = 0;
         }
     }
-    float largest;
-    bool any;
-    uint32_t nSlots;
-    Stats all = Pass<T, kThreads, kTop, false>(a, row, from, to, waveStats[0], waveMost, largest, any, groupMost, nSlots, token);
-    const float most = LaneMax(lane < kWaves ? waveMost[lane] : -__builtin_inff());     // of the workgroup
-    // (-inf alone leaves s = 0, or a NaN, in either form)
-    const bool safe = most != -__builtin_inff() && !(fabsf(most * a.exp2Scale) <= kReach);
-    if (__builtin_expect(safe, 0)) {
-        __syncthreads();      // (the maxima above are overwritten)
-        all = Pass<T, kThreads, kTop, true>(a, row, from, to, waveStats[1], waveMost, largest, any, groupMost, nSlots, token);
+    Stats acc = kNoElements;
+    Reader<T, kThreads> reader(a, row, from, to);
+    U32x4 raw[kUnroll];
+    uint32_t fetch = 0, slotMost = 0;
+    while (reader.Fetch(raw)) {
+        float x[kUnroll * P];
+        for (uint32_t u = 0; u < kUnroll; ++u) {
+            Unpack16<T>(raw[u], x + u * P);
+        }
+        if (fetch == 0) {
+            token.logit = TokenLogit<T>(a, row, token.id);      // on its way while the row is read
+        }
+        const float most = Accumulate<kUnroll * P>(acc, x, a.exp2Scale);
+        if constexpr (kTop) {
+            const uint32_t order = Ordered(most) >> 16;
+            slotMost = (fetch & ((1u << a.slotShift) - 1u)) != 0 && slotMost > order ? slotMost : order;
+            groupMost[(fetch >> a.slotShift) * kThreads + tid] = static_cast<uint16_t>(slotMost);
+        }
+        ++fetch;
     }
-    const RowResult result = Finish(all, safe, a);
+    const Stats wave = WaveJoin(acc, a.exp2Scale);
+    if (lane == 0) {
+        waveStats[tid / kWave] = wave;
+    }
+    __syncthreads();
+    const Stats all = WaveJoin(lane < kWaves ? waveStats[lane] : kNoElements, a.exp2Scale);
+    const RowResult result = Finish(all, a.scale);
     if constexpr (kTop) {
         if (!result.bad) {     // a NaN has no place in an order: no alternatives
-            GatherTop<T>(a, row, from, to, any ? Ordered(largest) : 0u, Ordered(most), nSlots, groupMost, sh, tid);
+            // (a lane, or a workgroup, that has met nothing but -inf still has the lowest finite value as its largest)
+            const float laneMost = acc.s == 0.0 ? -__builtin_inff() : acc.m, most = result.none ? -__builtin_inff() : all.m;
+            const uint32_t nSlots = (fetch + (1u << a.slotShift) - 1) >> a.slotShift;
+            GatherTop<T>(a, row, from, to, reader.any ? Ordered(laneMost) : 0u, Ordered(most), nSlots, groupMost, sh, tid);
         }
     }
     if (a.nSplit == 1) {
@@ -762,10 +724,7 @@ __global__ __launch_bounds__(kThreads, kThreads > 256 ? 4 : kTop ? 7 : 8) void L
     }
     const uint64_t at = row * a.nSplit + split;
     if (tid == 0) {
-        StoreOne(a.stats + at * 4, all.m);
-        StoreOne(a.stats + at * 4 + 1, all.s);
-        StoreOne(a.stats + at * 4 + 2, all.t);
-        StoreOne(a.stats + at * 4 + 3, !safe ? 1.0f : most < 0.0f ? 0.0f : 2.0f);
+        StoreOne(reinterpret_cast<U32x4*>(a.stats + at), __builtin_bit_cast(U32x4, all));
     }
     if constexpr (kTop) {
         if (tid < a.topCount) {
@@ -784,26 +743,15 @@ __global__ __launch_bounds__(kJoinThreads) void LogProbsJoinKernel(const LogProb
     const uint64_t row = blockIdx.x;
     Token token = {TokenId(a, row), 0.0f};
     // every wavefront joins the numbers for itself, a lane per split
-    Stats mine = NoElements<false>();
-    float reach = -1.0f;    // 0, 1, 2: the split's largest logit is far below, within, far above what `m` can be a multiple of
+    Stats mine = kNoElements;
     const uint64_t* keys = a.keys + row * a.nSplit * a.topCount;
     uint64_t last = 0;      // the lowest key of the lane's list
     if (lane < a.nSplit) {
-        const float* p = a.stats + (row * a.nSplit + lane) * 4;
-        mine = Stats{LoadOne(p), LoadOne(p + 1), LoadOne(p + 2)};
-        reach = mine.s != 0.0f ? LoadOne(p + 3) : -1.0f;
+        mine = __builtin_bit_cast(Stats, LoadOne(reinterpret_cast<const U32x4*>(a.stats + row * a.nSplit + lane)));
         last = a.topCount != 0 ? LoadOne(keys + static_cast<uint64_t>(lane) * a.topCount + a.topCount - 1) : 0;
     }
     token.logit = TokenLogit<T>(a, row, token.id);
-    // Splits of a lower class than the highest have no weight beside it (but a NaN in any shows).
-    const float highest = LaneMax(reach);
-    const bool safe = highest == 0.0f || highest == 2.0f, nan = __any(mine.s != mine.s);
-    if (reach != highest) {
-        mine = safe ? NoElements<true>() : NoElements<false>();
-    }
-    Stats all = safe ? WaveJoin<true>(mine, a.exp2Scale) : WaveJoin<false>(mine, a.exp2Scale);
-    all.s = nan ? __builtin_nanf("") : all.s;
-    const RowResult result = Finish(all, safe, a);
+    const RowResult result = Finish(WaveJoin(mine, a.exp2Scale), a.scale);
     __shared__ uint64_t top[kMaxTop];
     if (a.topCount != 0 && !result.bad) {
         // The largest topCount-th key of any list bounds the result from below: what is less drops out.

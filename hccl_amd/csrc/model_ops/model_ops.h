@@ -14,13 +14,19 @@ constexpr uint32_t kMaxShards = HCCL_AMD_MAX_RANKS;
 constexpr uint32_t kMaxTop = HCCL_AMD_MAX_TOP;
 
 // ---- log probabilities ----------------------------------------------------------------------------------------
+// Of a set of elements x: the largest, and with y = c (x - m), c = scale * log2(e), the sums of y 2^y and of 2^y.
+struct alignas(16) LogProbsStats {
+    float m, t;
+    double s;
+};
+
 // One row of logits is the concatenation of nShards parts.
 struct LogProbsArgs {
     const void* logits[kMaxShards];
     uint64_t rowStride[kMaxShards];     // elements
     uint32_t count[kMaxShards];         // elements of the part
     const void* tokens;
-    float* stats;           // nSplit > 1: [row][split][4] = reference, sum, weighted sum, class of the reference
+    LogProbsStats* stats;   // nSplit > 1: [row][split]
     uint64_t* keys;         //             [row][split][topCount], descending, 0 where there is none
     uint32_t nShards;
     uint32_t nSplit;        // workgroups per row

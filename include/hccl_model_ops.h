@@ -42,7 +42,7 @@ extern "C" {
  */
 typedef struct {
     const void* logits;       /* tokenCount rows of vocabCount elements, rowStride elements apart, element-aligned */
-    uint64_t rowStride;       /* >= vocabCount */
+    uint64_t rowStride;       /* >= vocabCount, at most 2^36 */
     uint64_t vocabStart;      /* index of this rank's first entry: the sum of vocabCount over the lower ranks */
     uint64_t vocabCount;      /* may differ between ranks, may be 0; V is 1 .. 2^31 - 1 */
     uint64_t tokenCount;      /* rows, the same on every rank, below 2^24; 0: nothing to do on any rank */

@@ -218,6 +218,45 @@ def test_masked_rows(worlds, dtype, t, v):
     assert got[4][0].tolist() == list(range(16)) and bool((got[3][0] == -math.inf).all())
 
 
+@pytest.mark.parametrize("t,v,ranks", [(400, 700, 1), (64, 2678, 4), (300, 32768, 2), (8, 131072, 3), (1, 20000, 1)])
+def test_a_likely_token_keeps_its_digits(worlds, t, v, ranks):
+    """All logits but one are equal, so that all their terms are one e, and that one's is 1: s = 1 + (V - 1) e, chosen between
+    1.02 and 1.05.  s is off by the three roundings of the eight terms next to the 1, at most 3 U (values below 2), and by
+    what is relative to (V - 1) e <= 0.05: e's own error, |y| 3 U + 2 U with |y| <= 15 log2 e, and three roundings, one by
+    one below 0.05 (65 + 2 + 3) U = 3.5 U.  Then ln s, a relative 4 U and ln s below 0.05, and one rounding."""
+    x = torch.zeros(t, v)
+    top = torch.randint(0, v, (t,), generator=torch.Generator().manual_seed(v))
+    share = 0.02 + 0.03 * torch.rand(t, generator=torch.Generator().manual_seed(t))
+    x[torch.arange(t), top] = ((v - 1) / share).log()
+    rows = Rows(x, DT.FP32, ranks, 2)
+    lp, lse, entropy, values, ids = rows.run(worlds(ranks), top)
+    exact = reference(rows.x, top, 1.0, 2)
+    assert bool(((lp - exact[0]).abs() <= 7 * U).all()), float((lp - exact[0]).abs().max() / U)
+    assert torch.equal(values[:, 0], lp) and torch.equal(ids[:, 0], top)
+
+
+@pytest.mark.parametrize("dtype", [DT.FP32, DT.BFP16, DT.FP16])
+@pytest.mark.parametrize("t,v,ranks", [(5, 40, 1), (4, 2678, 4), (130, 5001, 2), (300, 9000, 3), (1025, 700, 1), (1, 100000, 1)])
+def test_a_certain_token_has_probability_one(worlds, dtype, t, v, ranks):
+    """Every other logit lies at least 34 below the largest, so that all of them together add less than 10^5 e^-34 < 2^-32
+    to its term of exactly 1, and 0 <= ln s < 2^-32.  The largest one's log probability is then within 2^-32 of 0, that of
+    another the difference, rounded as a 32-bit subtraction rounds it (2^-32 is far below half its step), lse the logit
+    itself; the entropy is at most ln s plus the sum of |y| e^y, below 2^-32 (1 + 34 + 60)."""
+    x = rng_tensor(t + v, t, v, scale=2.0).clamp(-10, 10) - 40
+    top = torch.randint(0, v, (t,), generator=torch.Generator().manual_seed(v))
+    most = rng_tensor(t, t, scale=0.9).clamp(-3, 3) + 7.3
+    x[torch.arange(t), top] = most
+    rows = Rows(x, dtype, ranks, 3)
+    for tokens in (top, (top + v // 2) % v):
+        lp, lse, entropy, values, ids = rows.run(worlds(ranks), tokens)
+        m = rows.x.float()[torch.arange(t), top]
+        exact = (rows.x.float()[torch.arange(t), tokens] - m).double()
+        assert bool((torch.where(exact == 0, (lp <= 0) & (lp > -2.0 ** -32), lp == exact)).all())
+        assert torch.equal(lse, m.double())
+        assert torch.equal(ids[:, 0], top) and bool(((values[:, 0] <= 0) & (values[:, 0] > -2.0 ** -32)).all())
+        assert bool((entropy.abs() <= 2.0 ** -32 * 95).all())
+
+
 @pytest.mark.parametrize("t,v", [(1030, 8000), (3, 100000)])
 def test_many_equal_logits(worlds, t, v):
     """Rows in which far more entries reach the bound on the alternatives than its list holds: few values, one value, and
