@@ -59,9 +59,9 @@ def split(vocab, ranks, seed=0):
 
 class Rows:
     """Logits [T, V] of a type, dealt to ranks as parts that start on any element and whose rows are any distance apart,
-    and the outputs of every rank."""
+    and the outputs of every rank.  With `tight` a part's memory ends with its last element."""
 
-    def __init__(self, x, dtype, ranks, top=0, token_type=DT.INT64, parts=None, pad=3, offset=1):
+    def __init__(self, x, dtype, ranks, top=0, token_type=DT.INT64, parts=None, pad=3, offset=1, tight=False):
         self.t, self.v = x.shape
         self.dtype, self.top, self.token_type = dtype, top, token_type
         self.x = x.to(TORCH[dtype])
@@ -69,11 +69,9 @@ class Rows:
         self.shards = []
         for start, count in self.parts:
             stride = count + pad
-            room = torch.full((offset + self.t * stride + 8,), FILL, dtype=TORCH[dtype])
-            view = room[offset:offset + self.t * stride].view(self.t, stride)
-            view[:, :count] = self.x[:, start:start + count]
-            room = room.cuda()
-            self.shards.append(room[offset:offset + self.t * stride].view(self.t, stride))
+            room, whole = self.room(offset, stride, count if tight else stride)
+            whole[:, :count] = self.x[:, start:start + count].cuda()
+            self.shards.append(whole)
         n = len(self.parts)
         self.log_probs = [torch.full((self.t + 1,), FILL, device="cuda") for _ in range(n)]
         self.lse = [torch.full((self.t + 1,), FILL, device="cuda") for _ in range(n)]
@@ -81,10 +79,15 @@ class Rows:
         self.values = [torch.full((self.t * top + 1,), FILL, device="cuda") for _ in range(n)]
         self.ids = [torch.full((self.t * top + 1,), 77, device="cuda", dtype=TORCH[token_type]) for _ in range(n)]
 
+    def room(self, offset, stride, width):
+        """Memory of T rows `stride` apart, of which `width` elements are looked at, that ends with the last of these."""
+        room = torch.full((offset + (self.t - 1) * stride + width,), FILL, dtype=TORCH[self.dtype], device="cuda")
+        return room, room.as_strided((self.t, width), (stride, 1), offset)
+
     def run(self, w, tokens, scale=1.0, streams=None, space=None):
         tokens = tokens.to(TORCH[self.token_type]).cuda()
         size = model_ops.token_log_probs_workspace(self.t, self.v, self.top)
-        space = torch.full((size + 16,), 255, dtype=torch.uint8, device="cuda") if space is None else space
+        space = torch.full((max(size, 1),), 255, dtype=torch.uint8, device="cuda") if space is None else space
         torch.cuda.synchronize()
         with hccl_amd.group():
             for r, (start, count) in enumerate(self.parts):
@@ -332,7 +335,7 @@ def test_ranks_on_their_own_streams_and_a_shared_workspace_in_turn(worlds):
 
 
 # ---- their gradient ----------------------------------------------------------------------------------------------
-def grad_case(w, rows, tokens, scale, g, e, h, in_place=False, lse=None, entropy=None, ids=None):
+def grad_case(w, rows, tokens, scale, g, e, h, in_place=False, lse=None, entropy=None, ids=None, tight=False):
     """The gradient of every rank's part, joined, and the numbers it was computed from."""
     _, ref_lse, ref_entropy, _, ref_ids, _ = reference(rows.x, tokens, scale, rows.top)
     lse = (ref_lse if lse is None else lse).float()
@@ -344,9 +347,9 @@ def grad_case(w, rows, tokens, scale, g, e, h, in_place=False, lse=None, entropy
     out = []
     for r, (start, count) in enumerate(rows.parts):
         s = rows.shards[r]
-        pad = 0 if in_place else 5
-        room = torch.full((2 + rows.t * (s.shape[1] + pad) + 8,), FILL, dtype=s.dtype, device="cuda")
-        d = s if in_place else room[1:1 + rows.t * (s.shape[1] + pad)].view(rows.t, s.shape[1] + pad)
+        stride = s.stride(0) + 5
+        room, d = rows.room(1, stride, count if tight else stride)
+        d = s if in_place else d
         torch.cuda.synchronize()
         model_ops.token_log_probs_grad(w.comms[r], s, rows.t, start, count, d_tokens, d_lse, d_g, d, data_type=rows.dtype,
                                        token_type=rows.token_type, row_stride=s.stride(0), grad_row_stride=d.stride(0),
@@ -355,7 +358,7 @@ def grad_case(w, rows, tokens, scale, g, e, h, in_place=False, lse=None, entropy
         w.sync()
         assert bool((d[:, count:] == FILL).all())          # the room between the rows stays
         if not in_place:
-            assert float(room[0]) == FILL and bool((room[1 + d.numel():] == FILL).all())
+            assert float(room[0]) == FILL
         out.append(d[:, :count].cpu())
     return torch.cat(out, 1), lse.double(), entropy.double(), ids
 
@@ -495,13 +498,13 @@ def test_gradient_against_differences_of_the_forward_pass(worlds):
 
 
 # ---- gradient norm -------------------------------------------------------------------------------------------------
-def norm_case(w, per_rank, max_norm=1.0, scale=1.0):
+def norm_case(w, per_rank, max_norm=1.0, scale=1.0, behind=9):
     """per_rank: lists of (host tensor, type, element offset); returns every rank's (norm, factor)."""
     keep, descr = [], []
     for tensors in per_rank:
         mine = []
         for x, dtype, offset in tensors:
-            room = torch.full((offset + x.numel() + 9,), 1e4, dtype=TORCH[dtype], device="cuda")
+            room = torch.full((offset + x.numel() + behind,), 1e4, dtype=TORCH[dtype], device="cuda")
             room[offset:offset + x.numel()] = x.to(TORCH[dtype]).cuda()
             keep.append(room)
             mine.append((room[offset:], x.numel(), dtype))
@@ -569,6 +572,28 @@ def test_norm_is_the_same_every_time(worlds):
         assert torch.equal(norm_case(worlds(3), per_rank), first)
 
 
+@pytest.mark.parametrize("dtype", [DT.FP32, DT.BFP16, DT.FP16])
+def test_memory_that_ends_with_the_last_element(worlds, dtype):
+    """No byte behind a buffer is read or written either: the run of this test on the CPU (test_emulated_model_ops.py) looks
+    at every access."""
+    for t, v, ranks in ((1, 1, 1), (2, 7, 1), (3, 9, 3), (2, 2055, 2), (5, 8193, 1), (1, 40003, 3), (260, 300, 2)):
+        for offset in (0, 1):
+            x = rng_tensor(t + v, t, v)
+            tokens, top = given(t, v, 1), min(v, 5)
+            g, e, h = rng_tensor(1, t), rng_tensor(2, t), rng_tensor(3, t, top)
+            rows = Rows(x, dtype, ranks, top, pad=offset, offset=offset, tight=True)
+            check_rows(rows, rows.run(worlds(ranks), tokens), tokens, 1.0)
+            got, lse, entropy, ids = grad_case(worlds(ranks), rows, tokens, 1.0, g, e, h, tight=True)
+            check_grad(rows, got, lse, entropy, ids, tokens, 1.0, g, e, h)
+    per_rank = [[(rng_tensor(n, n), dtype, n % 3) for n in (1, 3, 8, 15, 8191, 8193)]]
+    norm, factor = norm_reference(per_rank, 1.0, 1.0)
+    got = norm_case(worlds(1), per_rank, behind=0)
+    assert abs(got[0] - norm) <= 2 * U * norm and abs(got[1] - factor) <= 2 * U * factor
+    for fp8 in (False, True):
+        for combo in [c for c in COMBOS if c[1] == dtype]:
+            run_adamw(worlds(1), [Tensor(n, combo, fp8, n, n % 3, behind=0) for n in (1, 3, 257, 1023, 4099)], fp8)
+
+
 # ---- AdamW -----------------------------------------------------------------------------------------------------------
 E4M3 = torch.float8_e4m3fn
 COMBOS = [(DT.FP32, DT.FP32, False), (DT.FP32, DT.BFP16, False), (DT.FP32, DT.FP16, False), (DT.BFP16, DT.BFP16, False),
@@ -579,8 +604,8 @@ COMBOS = [(DT.FP32, DT.FP32, False), (DT.FP32, DT.BFP16, False), (DT.FP32, DT.FP
 class Tensor:
     """One tensor's buffers, each at an element offset inside a larger one that has to stay as it was."""
 
-    def __init__(self, n, combo, fp8, seed, offset=0, fresh=False):
-        self.n, (self.param_type, self.grad_type, self.with_master), self.fp8 = n, combo, fp8
+    def __init__(self, n, combo, fp8, seed, offset=0, fresh=False, behind=8):
+        self.behind, self.n, (self.param_type, self.grad_type, self.with_master), self.fp8 = behind, n, combo, fp8
         self.rooms = {}
         blocks = -(-n // 256)
         w = rng_tensor(seed, n, scale=0.05)
@@ -611,7 +636,7 @@ class Tensor:
             self.place("exp_avg_sq", root.square(), offset)
 
     def place(self, name, x, offset):
-        room = torch.full((offset + x.numel() + 8,), 77, dtype=x.dtype, device="cuda")
+        room = torch.full((offset + x.numel() + self.behind,), 77, dtype=x.dtype, device="cuda")
         room[offset:offset + x.numel()] = x.cuda()
         self.rooms[name] = (room, offset, x.numel())
 
