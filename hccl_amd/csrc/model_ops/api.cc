@@ -391,7 +391,8 @@ HcclResult CheckAdamWConfig(const char* name, const HcclAmdAdamWConfig& c)
         return HCCL_E_NOT_SUPPORT;
     }
     const bool betas = c.beta1 >= 0 && c.beta1 < 1 && c.beta2 >= 0 && c.beta2 < 1;
-    if (!betas || !(c.eps >= 0) || !std::isfinite(c.eps) || !std::isfinite(c.weightDecay) ||
+    const bool eps = c.eps == 0 || (c.eps >= 0x1p-126 && std::isfinite(c.eps));      // (reciprocals of less are infinite)
+    if (!betas || !eps || !std::isfinite(c.weightDecay) ||
         (c.lrOnDevice == nullptr && !std::isfinite(c.lr)) || (c.stepOnDevice == nullptr && c.step == 0)) {
         Log(1, "%s: lr %g, betas %g %g, eps %g, weight decay %g, step %llu are out of range", name, c.lr, c.beta1, c.beta2,
             c.eps, c.weightDecay, (unsigned long long)c.step);

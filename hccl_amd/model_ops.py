@@ -8,8 +8,9 @@ to its collectives, over the communicators of this package.
 * :func:`adamw` -- one AdamW step over many tensors, with states in 32 bits or in FP8 blocks of 256 elements.
 
 Buffers are device pointers (integers, ctypes pointers or anything with ``data_ptr()``), counts are elements, ``stream``
-must not be null, and a failing call raises :class:`hccl_amd.HcclError`, as for the collectives.  Drive several ranks from
-one thread inside ``with hccl_amd.group():``.  What the arguments mean is written in the header.
+must not be null, and a failing call raises :class:`hccl_amd.HcclError`, as for the collectives.  Rows of logits and of
+their gradient may be any distance apart (``row_stride``); everything else is contiguous.  Drive several ranks from one
+thread inside ``with hccl_amd.group():``.  What the arguments mean is written in the header.
 """
 import ctypes
 import os

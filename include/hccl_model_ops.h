@@ -36,7 +36,7 @@ extern "C" {
  *   logSumExp[i]     lse
  *   entropy[i]       -sum(p log p), p = exp(x - lse)
  *   topIds[i][j]     the j-th most likely entry, the lower index of equal ones; topValues[i][j] = x[topIds[i][j]] - lse
- * Sums are kept in 32 bits, relative to the row's maximum.  -inf logits are entries that cannot occur.  A row of -inf
+ * Sums are kept in 32 bits or more, relative to the row's maximum.  -inf logits are entries that cannot occur.  A row of -inf
  * alone has logSumExp -inf, logProbs -inf (0 if ignored), entropy 0, topIds 0, 1, ... and topValues -inf.  A row with a
  * NaN or +inf has NaN in every output but topIds, which are -1, and the 0 of an ignored token.
  */
@@ -148,7 +148,7 @@ typedef struct {
 typedef struct {
     double lr;
     double beta1, beta2;      /* [0, 1) */
-    double eps;               /* >= 0 */
+    double eps;               /* >= 2^-126, or 0: elements whose v is 0, or below 2^-126, then have no defined step */
     double weightDecay;
     uint64_t step;            /* 1 for the first step */
     const int64_t* stepOnDevice;   /* null, or read instead of step when the kernels run (captured steps) */

@@ -191,7 +191,7 @@ def test_adamw(one):
     assert adamw(one, state_type=DT.FP8E5M2) == NOT_SUPPORT
     assert adamw(one, step=0) == PARA
     for bad in (dict(lr=math.nan), dict(beta1=1.0), dict(beta1=-0.1), dict(beta2=1.0), dict(beta2=math.nan), dict(eps=-1.0),
-                dict(eps=math.inf), dict(weight_decay=math.inf)):
+                dict(eps=math.inf), dict(eps=1e-40), dict(eps=math.nan), dict(weight_decay=math.inf)):
         assert adamw(one, **bad) == PARA, bad
     assert adamw(one, step_on_device=A + 4) == PARA
     assert adamw(one, lr_on_device=A + 2) == PARA
