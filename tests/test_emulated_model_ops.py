@@ -21,6 +21,7 @@ DESELECT = ["test_calls_can_be_captured_into_a_graph_and_replayed", "test_logits
 def environment(log):
     base, lib = build_model_ops.build()
     env = emu_env(base, log)
+    env["ASAN_OPTIONS"] += ":detect_stack_use_after_return=0"      # would map and unmap a stack of its own for every lane
     env["HCCL_AMD_TEST_EMU_MODEL_OPS_LIB"] = lib
     env["PYTHONPATH"] = os.pathsep.join([ROOT, os.path.join(ROOT, "tests"), os.path.join(ROOT, "tests", "emu"),
                                          env.get("PYTHONPATH", "")])
