@@ -5,10 +5,15 @@
 // exchanges between lanes and no memory.  m and v are updated in 32 bits and rounded once on the way out; the weights take
 // the unrounded ones.  Of v the root is stored: that halves the exponents it needs, and it is what the step divides by.  A
 // root above zero is stored as at least the smallest code: rounded to zero it would leave m / eps as a step.
-// Square root and reciprocal are the one-instruction forms (1 ulp): the step is 1e-7 of itself off, the weight far less.
+// The states' products and sums are rounded one by one, and on the way to codes the root and the quotients too: the states
+// are then the bits that elementwise 32-bit operations give.  One bit more or less can decide between two codes, 6 %
+// apart, and one step later between two scales.  (With fused operations and the one-instruction root, four steps on 2^27
+// weights left 1371 codes and two scales that were not the same; 1 % faster with FP8 states, equally fast with 32-bit
+// ones.)  In the weights' step the reciprocal, and with 32-bit states the root, are the one-instruction forms (1 ulp): it
+// is 1e-7 of itself off, the weight far less.
 //
 // Bound: every tensor read once and the updated ones written once.  2^27 bf16 weights in 300 tensors with 32-bit master
-// weights, four launches: 629 us, 6.0 TB/s of the 6.0 - 6.7 that a copy reaches; with FP8 states 379 us, 5.7 TB/s.  (A lane
+// weights, four launches: 625 us, 6.0 TB/s of the 6.0 - 6.7 that a copy reaches; with FP8 states 381 us, 5.7 TB/s.  (A lane
 // with eight neighbours, two 16-byte accesses 32 bytes apart: 790 and 486.  Chunks of 1024 elements 631 and 393, of 4096
 // 676 and 396; stores written through 651 and 391, plain ones 701 and 414.)
 #include "model_ops.h"
@@ -196,9 +201,9 @@ __global__ __launch_bounds__(kThreads) void AdamWKernel(const AdamWArgs a)
                 v[s][i] *= v[s][i];
             }
             const float gi = g[s][i] * clip;
-            m[s][i] = __builtin_fmaf(m[s][i], a.beta1, gi * a.oneMinusBeta1);
-            v[s][i] = __builtin_fmaf(v[s][i], a.beta2, gi * gi * a.oneMinusBeta2);
-            root[i] = __builtin_amdgcn_sqrtf(v[s][i]);
+            m[s][i] = m[s][i] * a.beta1 + gi * a.oneMinusBeta1;
+            v[s][i] = v[s][i] * a.beta2 + gi * gi * a.oneMinusBeta2;
+            root[i] = kFp8 ? sqrtf(v[s][i]) : __builtin_amdgcn_sqrtf(v[s][i]);
             const float step = m[s][i] * __builtin_amdgcn_rcpf(__builtin_fmaf(root[i], rootCorrection2, a.eps));
             w[s][i] = __builtin_fmaf(-rate, step, w[s][i] * keep);
             if constexpr (kMaster) {
@@ -214,14 +219,15 @@ __global__ __launch_bounds__(kThreads) void AdamWKernel(const AdamWArgs a)
                 root[i] = i < n ? root[i] : 0.0f;
             }
             const float mMost = BlockMax(m[s]), vMost = BlockMax(root);
-            const float mUnit = mMost > kNoUnit ? kCodeMax / mMost : 0.0f, vUnit = vMost > kNoUnit ? kCodeMax / vMost : 0.0f;
+            const float mUnit = mMost > kNoUnit ? 1.0f / mMost * kCodeMax : 0.0f;
+            const float vUnit = vMost > kNoUnit ? 1.0f / vMost * kCodeMax : 0.0f;
             for (uint32_t i = 0; i < kPer; ++i) {
                 m[s][i] *= mUnit;
                 root[i] = root[i] > 0.0f ? fmaxf(root[i] * vUnit, kCodeMin) : root[i];
             }
             if (n != 0 && threadIdx.x % kWave == 0) {
-                StoreOne(mScales + at / kBlock, mMost / kCodeMax);
-                StoreOne(vScales + at / kBlock, vMost / kCodeMax);
+                StoreOne(mScales + at / kBlock, mMost * (1.0f / kCodeMax));
+                StoreOne(vScales + at / kBlock, vMost * (1.0f / kCodeMax));
             }
         }
         if (n != 0) {

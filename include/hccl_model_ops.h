@@ -127,7 +127,7 @@ HcclResult HcclAmdGradNormWorkspace(uint64_t tensorCount, uint64_t* bytes);
  *   w = w (1 - lr weightDecay) - lr / (1 - beta1^step) * m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
  * in 32 bits.  w is `master` if given, else `param`; `param` receives w rounded to its type.
  * stateType FP32: expAvg = m and expAvgSq = v are floats.  stateType FP8E4M3: both are e4m3 codes in blocks of
- * HCCL_AMD_STATE_BLOCK elements (the last one short), each with a float scale = largest magnitude / 448: m = code * scale,
+ * HCCL_AMD_STATE_BLOCK elements (the last one short), each with a float scale = largest magnitude * (1 / 448): m = code * scale,
  * and expAvgSq holds the root of v, v = (code * scale)^2, of which a value above 0 is never rounded to 0.  The step uses m
  * and v before they are rounded.
  * The tensors of one call must not overlap.  Zero-filled states and scales are the start.

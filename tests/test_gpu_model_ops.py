@@ -767,6 +767,41 @@ def test_adamw_skips_a_step_whose_norm_is_not_finite(worlds):
         assert not torch.equal(t.host()["master"], before["master"])
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+def test_adamw_states_are_the_bits_of_elementwise_operations(worlds, fp8):
+    """m and v, or their codes and scales, over five steps: every product, sum, root and quotient rounded to 32 bits."""
+    n, beta1, beta2 = 256 * 1200 + 77, 0.9, 0.99
+    t = Tensor(n, (DT.BFP16, DT.BFP16, True), fp8, 11)
+    f = lambda x: torch.tensor(x, dtype=torch.float32)  # noqa: E731
+    host = t.host()
+    m, v = host["exp_avg"], host["exp_avg_sq"]
+    units = lambda x: x.repeat_interleave(256)[:n]  # noqa: E731
+    blocks = lambda x: torch.nn.functional.pad(x, (0, -n % 256)).view(-1, 256).abs().amax(1)  # noqa: E731
+    if fp8:
+        m, m_scale = m.view(E4M3).float(), host["exp_avg_scale"]
+        v, v_scale = v.view(E4M3).float(), host["exp_avg_sq_scale"]
+    for step in range(1, 6):
+        t.view("grad").copy_(rng_tensor(step, n, scale=0.01).to(torch.bfloat16))
+        g = t.host()["grad"].float() * f(0.37)
+        if fp8:
+            m, v = m * units(m_scale), (v * units(v_scale)).square()
+        m = m * f(beta1) + g * f(1 - beta1)
+        v = v * f(beta2) + g * g * f(1 - beta2)
+        run_adamw(worlds(1), [t], fp8, step=step, clip=0.37, check=False)
+        got = t.host()
+        if fp8:
+            root = v.double().sqrt().float()      # (rounds as the root in 32 bits: 53 bits are more than twice 24 and two)
+            most, most_root = blocks(m), blocks(root)
+            m_scale, v_scale = most * f(448.0).reciprocal(), most_root * f(448.0).reciprocal()
+            m = (m * units(most.reciprocal() * 448)).to(E4M3)
+            v = torch.where(root > 0, (root * units(most_root.reciprocal() * 448)).clamp(min=2.0 ** -9), 0.0).to(E4M3)
+            assert torch.equal(got["exp_avg_scale"], m_scale) and torch.equal(got["exp_avg_sq_scale"], v_scale), step
+            assert torch.equal(got["exp_avg"], m.view(torch.uint8)) and torch.equal(got["exp_avg_sq"], v.view(torch.uint8)), step
+            m, v = m.float(), v.float()
+        else:
+            assert torch.equal(got["exp_avg"], m) and torch.equal(got["exp_avg_sq"], v), step
+
+
 def test_adamw_quantises_as_the_type_says(worlds):
     """Codes of a block whose largest magnitude is 448 / 0.1: exactly the nearest e4m3 values, subnormal ones among them."""
     n = 4096
@@ -777,7 +812,7 @@ def test_adamw_quantises_as_the_type_says(worlds):
     run_adamw(worlds(1), [t], True, step=1, beta1=0.0, beta2=0.0)
     got = t.host()
     scale = got["exp_avg_scale"].repeat_interleave(256)
-    assert bool((scale == g.view(-1, 256).abs().amax(1).repeat_interleave(256) / 448).all())
+    assert bool((scale == g.view(-1, 256).abs().amax(1).repeat_interleave(256) * torch.tensor(448.0).reciprocal()).all())
     clean = g.view(-1, 256).abs().amax(1).repeat_interleave(256) == 448.0
     want = g.to(E4M3).view(torch.uint8)
     assert torch.equal(got["exp_avg"][clean], want[clean])
