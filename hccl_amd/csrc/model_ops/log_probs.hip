@@ -830,20 +830,22 @@ hipError_t Launch(LogProbsArgs& a, uint32_t rows, hipStream_t stream)
 
 // Measured on MI355X with bf16 rows, no alternatives / eight alternatives, in us (V = 8 vectors):
 //   rows x V        wave / row      256 / row       1024 / row      256, row split in
-//   4096 x 1000      7.4 / 11.5     17.6 / 25.1     71.6 / 122
-//   4096 x 16000    27.9 / 33.4     33.1 / 37.7     84.5 / 140
-//   4096 x 65536    89.5 / 97.4     88.8 / 93.7      117 / 175
-//   1024 x 4000      7.0 / 10.1      7.5 / 11.1     20.2 / 33.0
-//   1024 x 8000      9.4 / 12.8      8.6 / 12.1     21.9 / 35.7
-//    512 x 131072   69.1 / 78.1     27.0 / 31.7     29.6 / 37.2     29.8 / 35.2 (2)
-//    256 x 32768    19.2 / 24.0      8.7 / 12.2      8.2 / 11.4     10.0 / 14.5 (2)
-//    256 x 131072   66.5 / 75.8     22.2 / 27.1     16.4 / 20.2     18.2 / 23.4 (4)
-//    128 x 131072   65.8 / 75.2     20.9 / 26.0     13.4 / 17.4     12.7 / 17.6 (4)
-//     64 x 16000    10.5 / 13.8      6.3 / 9.0       6.9 / 10.3      7.5 / 12.0 (4)
-//     64 x 65536    34.0 / 40.2     12.0 / 16.2      8.7 / 12.5      8.5 / 13.1 (8)
-//     64 x 131072   65.2 / 74.1     20.5 / 25.5     13.0 / 17.1      9.9 / 14.7 (8)
-//     16 x 65536    27.7 / 33.7     11.1 / 14.5      8.5 / 12.0      7.2 / 11.4 (8)
-//      1 x 131072   42.9 / 51.0     13.5 / 17.9     11.2 / 14.8      6.5 / 11.0 (16)
+//   4096 x 1000      7.5 / 11.7     18.6 / 25.8     62.9 / 124
+//   4096 x 16000    29.4 / 34.3     33.6 / 38.5     64.9 / 144
+//   4096 x 65536    92.4 / 99.5     90.5 / 97.8      106 / 180
+//   1024 x 4000      7.0 / 10.1      7.6 / 11.2     18.5 / 34.0
+//   1024 x 8000      9.5 / 12.9      8.6 / 12.1     18.9 / 36.7
+//    512 x 131072   71.8 / 82.7     27.2 / 31.9     29.3 / 38.2     29.7 / 34.9 (2)
+//    256 x 32768    19.8 / 25.4      8.8 / 12.2      8.2 / 11.9      9.7 / 14.3 (2)
+//    256 x 131072   69.7 / 80.7     23.0 / 27.5     16.6 / 20.4     18.5 / 23.4 (4)
+//    128 x 131072   68.4 / 80.0     21.8 / 26.6     14.5 / 18.6     12.6 / 17.7 (4)
+//     64 x 16000    10.4 / 14.1      6.2 / 8.9       7.0 / 10.3      7.1 / 11.5 (4)
+//     64 x 65536    35.4 / 42.5     12.4 / 16.4      9.0 / 13.0      8.2 / 12.7 (8)
+//     64 x 131072   67.6 / 78.7     21.4 / 25.9     14.0 / 18.3      9.7 / 14.6 (8)
+//     16 x 65536    29.2 / 34.2     11.2 / 14.1      8.7 / 12.2      6.7 / 11.0 (8)
+//      1 x 131072   46.0 / 55.6     14.3 / 18.4     12.0 / 15.7      6.1 / 10.6 (16)
+// (Loading the next vectors before the present ones are summed: 4096 x 131072 175 against 174, 4096 x 16000 39 against 34,
+// 512 x 131072 25 against 27, with alternatives slower everywhere.)
 // A split row costs a second kernel of about 3 us, a workgroup of 1024 threads has a CU to itself.
 LogProbsForm LogProbsFormOf(uint64_t rows, uint64_t vectors)
 {
