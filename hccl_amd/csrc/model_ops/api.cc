@@ -232,7 +232,7 @@ HcclResult LaunchGradNorm(World* w, PendingOp& p, hipStream_t s)
             for (uint32_t i = nTensors; i < kNormBatch; ++i) {
                 a.chunkEnd[i] = 0xFFFFFFFFu;
             }
-            for (uint32_t i = 0; i < 16; ++i) {
+            for (uint32_t i = 0; i < 32; ++i) {
                 a.groupEnd[i] = i < kNormBatch / 16 ? a.chunkEnd[16 * i + 15] : 0xFFFFFFFFu;
             }
             HIP_OK(LaunchNormBatch(a, groups, s));
@@ -257,10 +257,10 @@ HcclResult LaunchGradNorm(World* w, PendingOp& p, hipStream_t s)
                 }
             }
             a.nChunks += static_cast<uint32_t>(chunks);
-            a.data[nTensors] = reinterpret_cast<const void*>(d[0]);
+            const uint64_t lastChunk = (d[1] - (chunks - 1) * perChunk) * DataTypeSize(type) - 1;
+            const uint64_t code = type == HCCL_DATA_TYPE_FP32 ? 0u : type == HCCL_DATA_TYPE_BFP16 ? 1u : 2u;
+            a.tensor[nTensors] = d[0] | (lastChunk << 2 | code) << kNormAddressBits;
             a.chunkEnd[nTensors] = a.nChunks;
-            a.lastChunk[nTensors] = static_cast<uint32_t>((d[1] - (chunks - 1) * perChunk) * DataTypeSize(type)) << 2 |
-                                    (type == HCCL_DATA_TYPE_FP32 ? 0u : type == HCCL_DATA_TYPE_BFP16 ? 1u : 2u);
             nTensors++;
         }
     }
@@ -352,8 +352,9 @@ HcclResult CheckNormTensors(const char* name, const HcclAmdNormTensor* tensors, 
             Log(1, "%s: data of tensor %u is nullptr", name, i);
             return HCCL_E_PTR;
         }
-        if (t.count >= 1ull << 40 || !Aligned(t.data, DataTypeSize(t.dataType))) {
-            Log(1, "%s: tensor %u has %llu elements or is not element-aligned", name, i, (unsigned long long)t.count);
+        if (t.count >= 1ull << 40 || !Aligned(t.data, DataTypeSize(t.dataType)) ||
+            reinterpret_cast<uint64_t>(t.data) >> kNormAddressBits != 0) {
+            Log(1, "%s: tensor %u has %llu elements, is not element-aligned or at no device address", name, i, (unsigned long long)t.count);
             return HCCL_E_PARA;
         }
     }

@@ -5,9 +5,11 @@
 // the number of elements costs accuracy.  A workgroup leaves one partial sum and a last workgroup adds them: which elements
 // meet in which order depends on the sizes alone.
 //
-// Bound: one read of the gradients.  1 GiB of bf16 in 960 tensors of eight ranks, four launches and the last one: 178 us, 6.0
-// TB/s of the 7.0 that a plain read reaches; about 4 us of each launch is its start and end.  (Chunks dealt round the
-// workgroups instead of in runs: 182 at best, since every step then passes a dozen tensors.)
+// Bound: one read of the gradients.  1 GiB of bf16 in 960 tensors of eight ranks, three launches and the last one: 173 us, 6.2
+// TB/s of the 7.0 that a plain read reaches; about 4 us of each launch is its start and end.  For that reason a tensor's
+// address and size share a word: 320 fit the arguments of a launch.  (240 with words of their own: 176 us, and 21 instead of
+// 18 for 856 tensors of 40 elements.  Chunks dealt round the workgroups instead of in runs: 182 at best with four launches,
+// since every step then passes a dozen tensors.)
 #include "model_ops.h"
 #include "vec.h"
 
@@ -88,16 +90,21 @@ __device__ __forceinline__ uint32_t EndedOf16(const uint32_t* end, uint32_t chun
     return n;
 }
 
+__device__ __forceinline__ const uint8_t* Address(uint64_t tensor)
+{
+    return reinterpret_cast<const uint8_t*>(tensor & ((1ull << kNormAddressBits) - 1));
+}
+
 __global__ __launch_bounds__(kThreads) void NormBatchKernel(const NormArgs a)
 {
     const uint32_t first = blockIdx.x * a.perGroup;
     const uint32_t last = first + a.perGroup < a.nChunks ? first + a.perGroup : a.nChunks;
     // The tensor of the first chunk, the first one that ends behind it: sixteen by sixteen, not one by one.
-    const uint32_t group = EndedOf16(a.groupEnd, first);
+    const uint32_t group = EndedOf16(a.groupEnd, first) + EndedOf16(a.groupEnd + 16, first);
     uint32_t tensor = 16 * group + EndedOf16(a.chunkEnd + 16 * group, first);
     uint32_t end = a.chunkEnd[tensor], start = tensor == 0 ? 0u : a.chunkEnd[tensor - 1];
-    const uint8_t* data = static_cast<const uint8_t*>(a.data[tensor]);
-    uint32_t code = a.lastChunk[tensor];
+    const uint8_t* data = Address(a.tensor[tensor]);
+    uint32_t code = static_cast<uint32_t>(a.tensor[tensor] >> kNormAddressBits);
     double sum = 0.0;
     U32x4 raw[kVecs];
     for (uint32_t chunk = first; chunk < last; ++chunk) {
@@ -105,11 +112,11 @@ __global__ __launch_bounds__(kThreads) void NormBatchKernel(const NormArgs a)
             ++tensor;
             start = end;
             end = a.chunkEnd[tensor];
-            data = static_cast<const uint8_t*>(a.data[tensor]);
-            code = a.lastChunk[tensor];
+            data = Address(a.tensor[tensor]);
+            code = static_cast<uint32_t>(a.tensor[tensor] >> kNormAddressBits);
         }
         const uint32_t type = code & 3u;
-        LoadChunk(data + static_cast<uint64_t>(chunk - start) * kNormChunkBytes, chunk + 1 == end ? code >> 2 : kNormChunkBytes,
+        LoadChunk(data + static_cast<uint64_t>(chunk - start) * kNormChunkBytes, chunk + 1 == end ? (code >> 2) + 1 : kNormChunkBytes,
                   type == 0 ? 4 : 2, raw);
         sum = type == 0 ? Squares<F32>(raw, sum) : type == 1 ? Squares<B16>(raw, sum) : Squares<F16>(raw, sum);
     }

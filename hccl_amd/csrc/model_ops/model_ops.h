@@ -89,19 +89,20 @@ hipError_t LaunchLogProbsGrad(const LogProbsGradArgs& args, HcclDataType dtype, 
 
 // ---- gradient norm ------------------------------------------------------------------------------------------------
 // A batch of tensors cut into chunks of kNormChunkBytes; workgroup b sums the chunks [b * perGroup, (b + 1) * perGroup).
-constexpr uint32_t kNormBatch = 240;            // tensors per launch, a multiple of 16
+constexpr uint32_t kNormBatch = 320;            // tensors per launch, a multiple of 16
+constexpr uint32_t kNormAddressBits = 48;       // of a device address
 constexpr uint32_t kNormGroups = 4096;          // partial sums per launch, at most
 constexpr uint32_t kNormChunkBytes = 16384;
 struct NormArgs {
-    const void* data[kNormBatch];
+    uint64_t tensor[kNormBatch];        // address, with (bytes of the last chunk - 1) << 2 | type (0 fp32, 1 bf16, 2 fp16) above
     uint32_t chunkEnd[kNormBatch];      // inclusive prefix of the chunk counts, the rest 0xFFFFFFFF
-    uint32_t lastChunk[kNormBatch];     // bytes of the tensor's last chunk, << 2 | type (0 fp32, 1 bf16, 2 fp16)
-    uint32_t groupEnd[16];              // chunkEnd of every sixteenth tensor, the last entry 0xFFFFFFFF
+    uint32_t groupEnd[32];              // chunkEnd of every sixteenth tensor, the rest 0xFFFFFFFF
     double* partial;                    // one per workgroup
     uint32_t nChunks;
     uint32_t perGroup;
 };
-static_assert(sizeof(NormArgs) <= 4096 && kNormBatch % 16 == 0 && kNormBatch / 16 < 16, "kernel arguments");
+static_assert(sizeof(NormArgs) <= 4096 && kNormBatch % 16 == 0 && kNormBatch / 16 < 32, "kernel arguments");
+static_assert(kNormChunkBytes <= 1u << 14, "a last chunk's bytes and type are 16 bits");
 struct NormJoinArgs {
     const double* partial;
     uint32_t nPartial;
