@@ -168,6 +168,7 @@ def test_norm(one):
     assert norm(one, [(A, 4, DT.FP32), (A, 4, DT.INT32)]) == NOT_SUPPORT
     assert norm(one, [(A + 2, 4, DT.FP32)]) == PARA
     assert norm(one, [(A, 1 << 40, DT.FP32)]) == PARA
+    assert norm(one, [(1 << 48, 4, DT.FP32)]) == PARA
     need = model_ops.grad_norm_workspace(1)
     assert norm(one, workspace=A, workspace_bytes=need - 1) == MEMORY
     assert model_ops.grad_norm_workspace(1000) > need
