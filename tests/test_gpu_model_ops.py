@@ -848,6 +848,41 @@ def test_logits_beyond_32_bits_of_elements(worlds):
     assert float(x[:8].float().abs().max()) < 1e-9
 
 
+def test_more_rows_than_a_launch_of_the_gradient_takes(worlds):
+    """2^23 + 5 rows of three logits, about the most a call may have: all of them against torch in 64 bits, on the GPU.
+    s <= 3 has a handful of roundings, log p and the gradient a few more: 16 U of the largest terms, |z| <= 20 and 20."""
+    t, v, top = (1 << 23) + 5, 3, 2
+    w = worlds(1)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(t, v, device="cuda", generator=g).mul_(3).clamp_(-10, 10)
+    tokens = torch.randint(0, v, (t,), device="cuda", dtype=torch.int32, generator=g)
+    lp, lse, entropy, ge = (torch.full((t + 1,), FILL, device="cuda") for _ in range(4))
+    values = torch.full((t + 1, top), FILL, device="cuda")
+    ids = torch.full((t + 1, top), 77, device="cuda", dtype=torch.int32)
+    d = torch.full((t + 1, v), FILL, device="cuda")
+    ge.normal_(generator=g).clamp_(-4, 4)
+    torch.cuda.synchronize()
+    model_ops.token_log_probs(w.comms[0], x, t, 0, v, tokens, lp, token_type=DT.INT32, lse=lse, entropy=entropy, top_count=top,
+                              top_values=values, top_ids=ids, stream=w.stream)
+    model_ops.token_log_probs_grad(w.comms[0], x, t, 0, v, tokens, lse, ge, d, token_type=DT.INT32, entropy=entropy,
+                                   grad_entropy=ge, top_count=top, top_ids=ids, grad_top_values=values, stream=w.stream)
+    w.sync()
+    for a in (lp, lse, entropy, values[:, 0], values[:, 1], d[:, 0], d[:, 2]):
+        assert float(a[-1]) == FILL
+    log_p = torch.log_softmax(x.double(), 1)
+    at = tokens.long()[:, None]
+    close = lambda a, b, bound: float((a[:t].double() - b).abs().max()) <= 16 * U * bound  # noqa: E731
+    assert close(lp, log_p.gather(1, at)[:, 0], 20) and close(lse, torch.logsumexp(x.double(), 1), 20)
+    assert close(entropy, -(log_p.exp() * log_p).sum(1), 20)
+    order = torch.sort(x, dim=1, descending=True, stable=True).indices[:, :top]
+    assert torch.equal(ids[:t].long(), order) and close(values, log_p.gather(1, order), 20)
+    gd, hd = ge[:t].double(), values[:t].double()
+    p = log_p.exp()
+    want = -p * (gd + hd.sum(1))[:, None] - gd[:, None] * p * (log_p + entropy[:t].double()[:, None])
+    want.scatter_add_(1, at, gd[:, None]).scatter_add_(1, order, hd)
+    assert close(d, want, 20 * 64)       # terms of up to 4 + 40 + 4 (20 + 2), each p 20 U off
+
+
 def test_tensors_beyond_32_bits_of_elements(worlds):
     n, tail = (1 << 32) + 1000, 3000
     w = worlds(1)
