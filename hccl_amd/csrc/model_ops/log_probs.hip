@@ -845,7 +845,8 @@ hipError_t Launch(LogProbsArgs& a, uint32_t rows, hipStream_t stream)
 //     16 x 65536    29.2 / 34.2     11.2 / 14.1      8.7 / 12.2      6.7 / 11.0 (8)
 //      1 x 131072   46.0 / 55.6     14.3 / 18.4     12.0 / 15.7      6.1 / 10.6 (16)
 // (Loading the next vectors before the present ones are summed: 4096 x 131072 175 against 174, 4096 x 16000 39 against 34,
-// 512 x 131072 25 against 27, with alternatives slower everywhere.)
+// 512 x 131072 25 against 27, with alternatives slower everywhere.  128 threads a row: 3 to 10 % faster than
+// the form taken for 2048 x 32000 and 16384 x 32000, up to 10 % slower for 4096 x 65536.)
 // A split row costs a second kernel of about 3 us, a workgroup of 1024 threads has a CU to itself.
 LogProbsForm LogProbsFormOf(uint64_t rows, uint64_t vectors)
 {
