@@ -9,8 +9,8 @@
 // are then the bits that elementwise 32-bit operations give.  One bit more or less can decide between two codes, 6 %
 // apart, and one step later between two scales.  (With fused operations and the one-instruction root, four steps on 2^27
 // weights left 1371 codes and two scales that were not the same; 1 % faster with FP8 states, equally fast with 32-bit
-// ones.)  In the weights' step the reciprocal, and with 32-bit states the root, are the one-instruction forms (1 ulp): it
-// is 1e-7 of itself off, the weight far less.
+// ones.)  In the weights' step the reciprocal is the one-instruction form (1 ulp): it is 1e-7 of itself off, the weight far
+// less.  The root is not: that form takes a v below 2^-126 as 0, which would leave m / eps as a step.  (Equally fast.)
 //
 // Bound: every tensor read once and the updated ones written once.  2^27 bf16 weights in 300 tensors with 32-bit master
 // weights, four launches: 625 us, 6.0 TB/s of the 6.0 - 6.7 that a copy reaches; with FP8 states 381 us, 5.7 TB/s.  (A lane
@@ -203,7 +203,7 @@ __global__ __launch_bounds__(kThreads) void AdamWKernel(const AdamWArgs a)
             const float gi = g[s][i] * clip;
             m[s][i] = m[s][i] * a.beta1 + gi * a.oneMinusBeta1;
             v[s][i] = v[s][i] * a.beta2 + gi * gi * a.oneMinusBeta2;
-            root[i] = kFp8 ? sqrtf(v[s][i]) : __builtin_amdgcn_sqrtf(v[s][i]);
+            root[i] = sqrtf(v[s][i]);
             const float step = m[s][i] * __builtin_amdgcn_rcpf(__builtin_fmaf(root[i], rootCorrection2, a.eps));
             w[s][i] = __builtin_fmaf(-rate, step, w[s][i] * keep);
             if constexpr (kMaster) {

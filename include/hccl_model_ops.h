@@ -148,7 +148,7 @@ typedef struct {
 typedef struct {
     double lr;
     double beta1, beta2;      /* [0, 1) */
-    double eps;               /* >= 2^-126, or 0: elements whose v is 0, or below 2^-126, then have no defined step */
+    double eps;               /* >= 2^-126, or 0: elements whose v is 0 then have no defined step */
     double weightDecay;
     uint64_t step;            /* 1 for the first step */
     const int64_t* stepOnDevice;   /* null, or read instead of step when the kernels run (captured steps) */

@@ -768,6 +768,26 @@ def test_adamw_skips_a_step_whose_norm_is_not_finite(worlds):
 
 
 @pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("eps", [0.0, 1e-30, 2.0 ** -126, 1e-8])
+def test_adamw_with_second_moments_below_the_smallest_normal_number(worlds, fp8, eps):
+    """Gradients so small that v = (1 - beta2) g^2 is subnormal: half a step is then 2^-150, and relative to v
+    2^-150 / v, of which the root, and with it the step m / root, takes half.  (One block of equal elements: an FP8 state's
+    code is the largest one, so that the unrounded step is what is looked at.)  The other roundings of the step are fewer
+    than 24, each U of it; 2^-126 stands for results that are subnormal themselves."""
+    n, beta1, beta2, lr = 256, 0.9, 0.999, 1.0
+    for exponent in (-59, -61, -64, -67):
+        t = Tensor(n, (DT.FP32, DT.FP32, False), fp8, 1, fresh=True)
+        t.view("param").zero_()
+        g = torch.full((n,), 1.5 * 2.0 ** exponent)
+        t.view("grad").copy_(g)
+        run_adamw(worlds(1), [t], fp8, 1, lr, beta1, beta2, eps, 0.0, check=False)
+        v = (1 - beta2) * g.double() ** 2
+        assert 2.0 ** -148 < float(v[0]) < 2.0 ** -126
+        update = lr * g.double() / (g.double().abs() + eps)
+        assert bool(((t.view("param").cpu().double() + update).abs() <= (24 * U + 2.0 ** -150 / v) * update + 2.0 ** -126).all())
+
+
+@pytest.mark.parametrize("fp8", [False, True])
 def test_adamw_states_are_the_bits_of_elementwise_operations(worlds, fp8):
     """m and v, or their codes and scales, over five steps: every product, sum, root and quotient rounded to 32 bits."""
     n, beta1, beta2 = 256 * 1200 + 77, 0.9, 0.99
