@@ -8,7 +8,8 @@ to its collectives, over the communicators of this package.
 * :func:`adamw` -- one AdamW step over many tensors, with states in 32 bits or in FP8 blocks of 256 elements.
 
 Buffers are device pointers (integers, ctypes pointers or anything with ``data_ptr()``), counts are elements, ``stream``
-must not be null, and a failing call raises :class:`hccl_amd.HcclError`, as for the collectives.  Rows of logits and of
+must not be null, and a failing call raises :class:`hccl_amd.HcclError`, as for the collectives; a number that no field of
+the C structures holds is refused like any other, and the peers of a collective are released.  Rows of logits and of
 their gradient may be any distance apart (``row_stride``); everything else is contiguous.  Drive several ranks from one
 thread inside ``with hccl_amd.group():``.  What the arguments mean is written in the header.
 """
@@ -17,7 +18,7 @@ import os
 import struct
 
 import hccl_amd
-from hccl_amd import HcclDataType, _as_ptr, _as_stream, check
+from hccl_amd import HcclDataType, HcclError, HcclResult, _as_ptr, _as_stream, check
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libhccl_amd_model_ops.so")
@@ -75,6 +76,8 @@ _pack_grad = _packer(TokenLogProbsGradArgs)
 _pack_config = _packer(AdamWConfig)
 _pack_norm = _packer(NormTensor)
 _pack_adamw = _packer(AdamWTensor)
+_pack_size = struct.Struct("Q").pack
+_ANY_STREAM, _ANY_RESULT = ctypes.c_void_p(1), ctypes.c_void_p(4)      # of calls that are refused before they are looked at
 _ADAMW_FIELDS = frozenset(("param", "grad", "exp_avg", "exp_avg_sq", "master", "exp_avg_scale", "exp_avg_sq_scale", "count",
                            "param_type", "grad_type"))
 _lib = None
@@ -116,6 +119,14 @@ def _address(buf):
         return buf if isinstance(buf, int) else _as_ptr(buf).value or 0
 
 
+def _unfit(where, error, code=0):
+    """Raises for a call whose arguments could not be converted: a number that its field does not hold is a parameter error
+    like any other bad one, what is no number or buffer at all keeps the error that says so."""
+    if isinstance(error, struct.error):
+        raise HcclError(code or HcclResult.E_PARA, where) from error
+    raise error
+
+
 def token_log_probs_workspace(token_count, vocab_size, top_count=0):
     """Bytes of workspace a token_log_probs call over `token_count` rows of `vocab_size` entries (all ranks') needs."""
     size = ctypes.c_uint64()
@@ -130,11 +141,19 @@ def token_log_probs(hccl_comm, logits, token_count, vocab_start, vocab_count, to
                     stream=None):
     """Log probabilities of `tokens` under softmax(scale * logits), whose columns vocab_start .. vocab_start + vocab_count
     this rank holds; every output (log_probs, lse, entropy, top_values, top_ids) may be None."""
-    args = _pack_log_probs(_address(logits), vocab_count if row_stride is None else row_stride, vocab_start, vocab_count,
-                           token_count, _address(tokens), data_type, token_type, scale, top_count, _address(log_probs),
-                           _address(lse), _address(entropy), _address(top_values), _address(top_ids),
-                           _address(workspace), workspace_bytes)
-    return check(lib().HcclAmdTokenLogProbs(args, hccl_comm, _as_stream(stream)), "HcclAmdTokenLogProbs")
+    try:
+        args = _pack_log_probs(_address(logits), vocab_count if row_stride is None else row_stride, vocab_start, vocab_count,
+                               token_count, _address(tokens), data_type, token_type, scale, top_count,
+                               _address(log_probs), _address(lse), _address(entropy), _address(top_values),
+                               _address(top_ids), _address(workspace), workspace_bytes)
+        code = lib().HcclAmdTokenLogProbs(args, hccl_comm, _as_stream(stream))
+    except Exception as e:
+        # (The library itself raises nothing: it has not been entered.)  The rank takes its place among the
+        # collectives all the same, with a call that is refused: its peers return at once.  Without rows no rank takes one.
+        rows = 0 if isinstance(token_count, int) and token_count == 0 else 2 ** 64 - 1
+        args = _pack_log_probs(0, 0, 0, 0, rows, 0, HcclDataType.FP32, HcclDataType.INT64, 1.0, 0, 0, 0, 0, 0, 0, 0, 0)
+        _unfit("HcclAmdTokenLogProbs", e, lib().HcclAmdTokenLogProbs(args, hccl_comm, _ANY_STREAM))
+    return check(code, "HcclAmdTokenLogProbs")
 
 
 def token_log_probs_grad(hccl_comm, logits, token_count, vocab_start, vocab_count, tokens, lse, grad_log_probs, grad_logits,
@@ -143,17 +162,23 @@ def token_log_probs_grad(hccl_comm, logits, token_count, vocab_start, vocab_coun
                          grad_top_values=None, stream=None):
     """Writes the gradient with respect to this rank's part of the logits to `grad_logits` (which may be the logits
     themselves); local to the rank."""
-    args = _pack_grad(_address(logits), vocab_count if row_stride is None else row_stride, vocab_start, vocab_count,
-                      token_count, _address(tokens), data_type, token_type, scale, top_count, _address(lse),
-                      _address(entropy), _address(grad_log_probs), _address(grad_entropy), _address(top_ids),
-                      _address(grad_top_values), _address(grad_logits),
-                      vocab_count if grad_row_stride is None else grad_row_stride)
+    try:
+        args = _pack_grad(_address(logits), vocab_count if row_stride is None else row_stride, vocab_start, vocab_count,
+                          token_count, _address(tokens), data_type, token_type, scale, top_count, _address(lse),
+                          _address(entropy), _address(grad_log_probs), _address(grad_entropy), _address(top_ids),
+                          _address(grad_top_values), _address(grad_logits),
+                          vocab_count if grad_row_stride is None else grad_row_stride)
+    except struct.error as e:
+        _unfit("HcclAmdTokenLogProbsGrad", e)
     return check(lib().HcclAmdTokenLogProbsGrad(args, hccl_comm, _as_stream(stream)), "HcclAmdTokenLogProbsGrad")
 
 
 def norm_tensors(tensors):
     """The array grad_norm takes, from (buffer, count, data type) triples; it can be kept while the buffers stay."""
-    items = [_pack_norm(_address(buf), count, data_type) for buf, count, data_type in tensors]
+    try:
+        items = [_pack_norm(_address(buf), count, data_type) for buf, count, data_type in tensors]
+    except struct.error as e:
+        _unfit("norm_tensors", e)
     return (NormTensor * len(items)).from_buffer_copy(b"".join(items))
 
 
@@ -167,10 +192,17 @@ def grad_norm_workspace(tensor_count):
 def grad_norm(hccl_comm, tensors, max_norm, result, scale=1.0, workspace=None, workspace_bytes=0, stream=None):
     """result[0] = |scale| * 2-norm of all tensors of all ranks, result[1] = scale * the factor that brings it to
     `max_norm` (max_norm <= 0: no clipping).  `tensors`: what norm_tensors returned, or its argument."""
-    if not isinstance(tensors, ctypes.Array):
-        tensors = norm_tensors(tensors)
-    return check(lib().HcclAmdGradNorm(tensors, len(tensors), max_norm, scale, _as_ptr(result), _as_ptr(workspace),
-                                       workspace_bytes, hccl_comm, _as_stream(stream)), "HcclAmdGradNorm")
+    try:
+        if not (isinstance(tensors, ctypes.Array) and tensors._type_ is NormTensor):
+            tensors = norm_tensors(tensors)
+        _pack_size(workspace_bytes)      # (ctypes would take -1 for a very large workspace)
+        code = lib().HcclAmdGradNorm(tensors, len(tensors), max_norm, scale, _as_ptr(result), _as_ptr(workspace),
+                                     workspace_bytes, hccl_comm, _as_stream(stream))
+    except Exception as e:
+        # as in token_log_probs
+        _unfit("HcclAmdGradNorm", e, lib().HcclAmdGradNorm(None, 0, float("nan"), 1.0, _ANY_RESULT, None, 0, hccl_comm,
+                                                           _ANY_STREAM))
+    return check(code, "HcclAmdGradNorm")
 
 
 def adamw_tensors(tensors):
@@ -180,9 +212,12 @@ def adamw_tensors(tensors):
     for t in tensors:
         if not _ADAMW_FIELDS.issuperset(t):
             raise TypeError("adamw_tensors: unknown fields %s" % sorted(set(t) - _ADAMW_FIELDS))
-        items.append(_pack_adamw(_address(t["param"]), _address(t["grad"]), _address(t["exp_avg"]), _address(t["exp_avg_sq"]),
-                                 _address(t.get("master")), _address(t.get("exp_avg_scale")),
-                                 _address(t.get("exp_avg_sq_scale")), t["count"], t["param_type"], t["grad_type"]))
+        try:
+            items.append(_pack_adamw(_address(t["param"]), _address(t["grad"]), _address(t["exp_avg"]),
+                                     _address(t["exp_avg_sq"]), _address(t.get("master")), _address(t.get("exp_avg_scale")),
+                                     _address(t.get("exp_avg_sq_scale")), t["count"], t["param_type"], t["grad_type"]))
+        except struct.error as e:
+            _unfit("adamw_tensors", e)
     return (AdamWTensor * len(items)).from_buffer_copy(b"".join(items))
 
 
@@ -191,8 +226,11 @@ def adamw(hccl_comm, tensors, step, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight
           stream=None):
     """One AdamW step over all `tensors` (what adamw_tensors returned, or its argument); local to the rank.  `clip` is a
     grad_norm result; `step` counts from 1 (step_on_device: an int64 on the device that is read instead)."""
-    if not isinstance(tensors, ctypes.Array):
+    if not (isinstance(tensors, ctypes.Array) and tensors._type_ is AdamWTensor):
         tensors = adamw_tensors(tensors)
-    config = _pack_config(lr, beta1, beta2, eps, weight_decay, step, _address(step_on_device), _address(lr_on_device),
-                          _address(clip), state_type, 1 if skip_non_finite else 0)
+    try:
+        config = _pack_config(lr, beta1, beta2, eps, weight_decay, step, _address(step_on_device), _address(lr_on_device),
+                              _address(clip), state_type, 1 if skip_non_finite else 0)
+    except struct.error as e:
+        _unfit("HcclAmdAdamW", e)
     return check(lib().HcclAmdAdamW(tensors, len(tensors), config, hccl_comm, _as_stream(stream)), "HcclAmdAdamW")

@@ -254,6 +254,81 @@ def test_ranks_that_do_not_fit_together():
     assert adamw(comms[1]) == PARA
 
 
+def unfit_calls():
+    """(operator, arguments) that no field of the C structures holds, or that are no numbers or buffers at all."""
+    for k in (dict(token_count=-1), dict(token_count=1 << 64), dict(token_count=None), dict(vocab_count=-1),
+              dict(vocab_start=-1), dict(row_stride=-1), dict(top_count=1 << 32), dict(top_count=-1), dict(scale=1e39),
+              dict(scale="warm"), dict(data_type=1 << 40), dict(logits=-A), dict(logits=object()), dict(stream="x"),
+              dict(workspace=A, workspace_bytes=-1), dict(workspace=A, workspace_bytes=1 << 64)):
+        yield log_probs, k
+    for k in (dict(tensors=[(A, -1, DT.FP32)]), dict(tensors=[(A, 4, 1 << 40)]), dict(tensors=[(A, 4)]),
+              dict(tensors=[(object(), 4, DT.FP32)]), dict(max_norm=1e39), dict(max_norm=None), dict(scale="warm"),
+              dict(result=object()), dict(stream="x"), dict(workspace=A, workspace_bytes=-1),
+              dict(workspace=A, workspace_bytes=1 << 64)):
+        yield norm, k
+
+
+@pytest.mark.parametrize("call,bad", list(unfit_calls()))
+@pytest.mark.parametrize("rank", [0, 1])
+def test_a_call_whose_arguments_do_not_fit_releases_its_peers(call, bad, rank):
+    """It raises, HcclError where it is a number that is out of range, its peer gets the same code at once, within a group or from
+    a thread, and the collective that follows pairs up."""
+    comms = hccl_amd.comm_init_all(2)
+    try:
+        for grouped in (False, True):
+            got = {}
+
+            def go(r, k):
+                try:
+                    got[r] = call(comms[r], **k)
+                except Exception as e:
+                    got[r] = e
+            if grouped:
+                hccl_amd.group_start()
+                go(1 - rank, {})
+                go(rank, bad)
+                ended = code(hccl_amd.group_end)
+                assert ended in (OK, PARA)
+                assert got[1 - rank] == PARA or ended == PARA
+            else:
+                threads = [threading.Thread(target=go, args=(r, k), daemon=True) for r, k in ((rank, bad), (1 - rank, {}))]
+                for t in threads:
+                    t.start()
+                for t in threads:
+                    t.join(20)
+                assert got.get(1 - rank) == PARA, got
+            assert got[rank] == PARA or isinstance(got[rank], (TypeError, ValueError, ctypes.ArgumentError)), got
+        # nothing to launch, but both ranks have to be at the same place of the sequence
+        hccl_amd.group_start()
+        assert log_probs(comms[0], log_probs=None, vocab_start=0) == OK
+        assert log_probs(comms[1], log_probs=None, vocab_start=8) == OK
+        assert code(hccl_amd.group_end) == OK
+    finally:
+        for c in comms:
+            hccl_amd.comm_destroy(c)
+
+
+def test_unfit_numbers_raise_the_library_s_error(one):
+    """Not the packing's, and the local operators and the kept arrays too."""
+    for call, bad in unfit_calls():
+        if all(isinstance(v, (int, float)) for v in bad.values()):
+            assert call(one, **bad) == PARA, bad
+    assert log_probs(one, token_count=0, row_stride=-1) == PARA
+    assert log_probs(one, data_type=DT.FP64) == NOT_SUPPORT
+    for k in (dict(token_count=-1), dict(row_stride=-1), dict(grad_row_stride=1 << 64), dict(top_count=-1), dict(grad_logits=-A),
+              dict(data_type=1 << 40)):
+        assert grad(one, **k) == PARA, k
+    for k in (dict(step=-1), dict(step=1 << 64), dict(clip=-A)):
+        assert adamw(one, **k) == PARA, k
+    assert adamw(one, dict(count=-1)) == PARA
+    assert code(model_ops.adamw_tensors, [dict(param=A, grad=A, exp_avg=A, exp_avg_sq=A, count=-1, param_type=4, grad_type=4)]) == PARA
+    assert code(model_ops.norm_tensors, [(A, -1, DT.FP32)]) == PARA
+    # an array of the other operator's descriptors is none of this one's
+    kept = model_ops.adamw_tensors([dict(param=A, grad=A, exp_avg=A, exp_avg_sq=A, count=1, param_type=4, grad_type=4)])
+    with pytest.raises(TypeError):
+        model_ops.grad_norm(one, kept, 1.0, A, stream=STREAM)
+
+
 def test_a_broken_environment_fails_these_calls_too(monkeypatch):
     monkeypatch.setenv("HCCL_DETERMINISTIC", "perhaps")
     comms = hccl_amd.comm_init_all(1)
