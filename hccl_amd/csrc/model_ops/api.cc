@@ -570,6 +570,29 @@ HcclResult HcclAmdTokenLogProbsGrad(const HcclAmdTokenLogProbsGradArgs* args, Hc
             Log(1, "%s: gradLogits overlaps the logits without being them", name);
             return HCCL_E_PARA;
         }
+        // What a workgroup reads of its row, others may still need when it writes.
+        const uint64_t ids = a.tokenCount * a.topCount, pitch = a.gradRowStride * size;
+        const struct {
+            const void* data;
+            uint64_t bytes;
+        } read[] = {{a.logSumExp, 4 * a.tokenCount},
+                    {a.gradLogProbs != nullptr ? a.tokens : nullptr, idSize * a.tokenCount},
+                    {a.gradLogProbs, 4 * a.tokenCount},
+                    {a.gradEntropy != nullptr ? a.entropy : nullptr, 4 * a.tokenCount},
+                    {a.gradEntropy, 4 * a.tokenCount},
+                    {top ? a.topIds : nullptr, idSize * ids},
+                    {top ? a.gradTopValues : nullptr, 4 * ids}};
+        for (const auto& r : read) {
+            const uint64_t at = reinterpret_cast<uint64_t>(r.data);
+            if (r.data == nullptr || at >= dEnd || at + r.bytes <= d) {
+                continue;
+            }
+            const bool between = at >= d && (at - d) % pitch >= row && (at - d) % pitch + r.bytes <= pitch;
+            if (!between) {
+                Log(1, "%s: gradLogits overlaps an array that the rows' numbers are read from", name);
+                return HCCL_E_PARA;
+            }
+        }
         rc = CheckLocal(name, ref);
         if (rc != HCCL_SUCCESS) {
             return rc;

@@ -72,10 +72,10 @@ HcclResult HcclAmdTokenLogProbsWorkspace(uint64_t tokenCount, uint64_t vocabSize
  * with respect to this rank's part of the logits, given the forward pass's logSumExp, entropy and topIds:
  *   gradLogits[i][v] = scale * ([v = tokens[i]] g_i + sum_j [v = topIds[i][j]] h_ij - p_v (a_i + e_i (log p_v + entropy_i)))
  *   a_i = g_i + sum_j h_ij, g_i = 0 for a negative token; a token or topId >= V is not checked for and counts in a_i only
- * rounded once to dataType.  gradLogits may be the logits themselves (same address and stride); other overlaps are
- * refused where the call can see them.  A row whose incoming gradients are all 0 gets zeros whatever its logits are; so
- * does a row with logSumExp < -1e30, which -inf or the lowest finite value fills.  A negative topId is skipped with
- * its gradient.
+ * rounded once to dataType.  gradLogits may be the logits themselves (same address and stride); other overlaps, with the
+ * logits or with an array that is read for the rows, are refused.  A row whose incoming gradients are all 0 gets zeros
+ * whatever its logits are; so does a row with logSumExp < -1e30, which -inf or the lowest finite value fills.  A negative
+ * topId is skipped with its gradient.
  */
 typedef struct {
     const void* logits;

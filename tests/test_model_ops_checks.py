@@ -157,6 +157,28 @@ def test_grad(one):
     assert grad(one, row_stride=16, grad_row_stride=16, grad_logits=A + 14) == PARA
 
 
+@pytest.mark.parametrize("which", ["tokens", "lse", "grad_log_probs", "entropy", "grad_entropy", "top_ids", "grad_top_values"])
+def test_the_gradient_is_not_written_over_what_its_rows_are_computed_from(one, which):
+    """Three rows of 8 floats, 20 floats apart, at D; every array but one lies elsewhere."""
+    d = 0x90000
+    entry = 8 if which in ("tokens", "top_ids") else 4
+    size = 3 * entry * (2 if which.startswith(("top", "grad_top")) else 1)
+    arrays = dict(tokens=A, lse=A, grad_log_probs=A, entropy=A, grad_entropy=A, top_ids=A, grad_top_values=A)
+    row, stride, rows = 32, 80, 2 * 80 + 32
+    for at in (d - size + entry, d, d + 24, d + stride, d + stride - entry, d + rows - entry):
+        k = dict(arrays, **{which: at})
+        assert grad(one, logits=A + 0x1000, grad_logits=d, grad_row_stride=20, top_count=2, **k) == PARA, (which, at - d)
+    comms = hccl_amd.comm_init_all(2)      # a destroyed world refuses what passes the checks, before any launch
+    hccl_amd.comm_destroy(comms[0])
+    for at in (d - size, d + row, d + stride + row, d + stride - size, d + rows):
+        if at % entry == 0:
+            k = dict(arrays, **{which: at})
+            assert grad(comms[1], logits=A + 0x1000, grad_logits=d, grad_row_stride=20, top_count=2, **k) == UNAVAIL, (which, at - d)
+    # what is not read does not matter
+    assert grad(comms[1], logits=A + 0x1000, grad_logits=d, tokens=d, grad_log_probs=None, entropy=A, grad_entropy=A) == UNAVAIL
+    hccl_amd.comm_destroy(comms[1])
+
+
 def test_norm(one):
     assert norm(one, result=None) == PTR
     assert norm(one, result=A + 2) == PARA
