@@ -36,9 +36,10 @@ extern "C" {
  *   logSumExp[i]     lse
  *   entropy[i]       -sum(p log p), p = exp(x - lse)
  *   topIds[i][j]     the j-th most likely entry, the lower index of equal ones; topValues[i][j] = x[topIds[i][j]] - lse
- * Sums are kept in 32 bits or more, relative to the row's maximum.  -inf logits are entries that cannot occur.  A row of -inf
- * alone has logSumExp -inf, logProbs -inf (0 if ignored), entropy 0, topIds 0, 1, ... and topValues -inf.  A row with a
- * NaN or +inf has NaN in every output but topIds, which are -1, and the 0 of an ignored token.
+ * Sums are kept in 32 bits or more, relative to the row's maximum: a log p near 0 is right to 3 * 2^-24, not to 24 bits of
+ * its own.  -inf logits are entries that cannot occur.  A row of -inf alone has logSumExp -inf, logProbs -inf (0 if
+ * ignored), entropy 0, topIds 0, 1, ... and topValues -inf.  A row with a NaN or +inf has NaN in every output but topIds,
+ * which are -1, and the 0 of an ignored token.
  */
 typedef struct {
     const void* logits;       /* tokenCount rows of vocabCount elements, rowStride elements apart, element-aligned */

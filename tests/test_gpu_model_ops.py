@@ -238,6 +238,24 @@ def test_a_likely_token_keeps_its_digits(worlds, t, v, ranks):
     assert torch.equal(values[:, 0], lp) and torch.equal(ids[:, 0], top)
 
 
+@pytest.mark.parametrize("t,v,ranks", [(300, 1000, 1), (64, 4096, 2), (300, 32768, 1), (8, 131072, 3)])
+@pytest.mark.parametrize("share", [1e-3, 1e-4, 1e-5, 1e-6])
+def test_how_near_a_very_likely_token_comes(worlds, t, v, ranks, share):
+    """As above with s - 1 = share: three roundings next to the 1, 3 U, stay however small ln s is.  The others' terms are off
+    by what y and their carrying over to a larger maximum are, 3 U of either's exponent, and two exponentials, 2 U each; five
+    roundings of their sums; ln s and the result are off by 6 U of themselves."""
+    x = torch.zeros(t, v)
+    top = torch.randint(0, v, (t,), generator=torch.Generator().manual_seed(v))
+    y = ((v - 1) / (share * (0.7 + 0.6 * torch.rand(t, generator=torch.Generator().manual_seed(t))))).log()
+    x[torch.arange(t), top] = y
+    rows = Rows(x, DT.FP32, ranks, 2)
+    lp, lse, entropy, values, ids = rows.run(worlds(ranks), top)
+    exact = reference(rows.x, top, 1.0, 2)
+    tol = 3 * U + 1.3 * share * (6 * y.double() / math.log(2) + 9) * U + 6 * U * exact[0].abs()
+    assert bool(((lp - exact[0]).abs() <= tol).all()), float(((lp - exact[0]).abs() / tol).max())
+    assert torch.equal(values[:, 0], lp) and torch.equal(ids[:, 0], top)
+
+
 @pytest.mark.parametrize("dtype", [DT.FP32, DT.BFP16, DT.FP16])
 @pytest.mark.parametrize("t,v,ranks", [(5, 40, 1), (4, 2678, 4), (130, 5001, 2), (300, 9000, 3), (1025, 700, 1), (1, 100000, 1)])
 def test_a_certain_token_has_probability_one(worlds, dtype, t, v, ranks):
