@@ -77,6 +77,8 @@ HcclResult HcclAmdTokenLogProbsWorkspace(uint64_t tokenCount, uint64_t vocabSize
  * logits or with an array that is read for the rows, are refused.  A row whose incoming gradients are all 0 gets zeros
  * whatever its logits are; so does a row with logSumExp < -1e30, which -inf or the lowest finite value fills.  A negative
  * topId is skipped with its gradient.
+ * log p is formed from the 32-bit logSumExp: it is up to |logSumExp| * 2^-24 off, and p by that share of itself, which next
+ * to a p near 1 is also what 1 - p is off by.
  */
 typedef struct {
     const void* logits;

@@ -485,6 +485,32 @@ def test_gradient_of_masked_rows(worlds, dtype):
         assert bool((grad_case(worlds(1), lowest, torch.tensor([3]), 1.0, one, one, None)[0] == 0).all())
 
 
+@pytest.mark.parametrize("most", [5.0, 20.0, 40.0, 60.0, 1000.0, -300.0])
+@pytest.mark.parametrize("share", [1e-2, 1e-5])
+def test_gradient_of_likely_tokens_after_the_forward_pass(worlds, most, share):
+    """Forward, then backward with what it left, against the gradient in 64 bits, at a large log-sum-exp and 1 - p = share.  The
+    backward pass takes log p from the 32-bit lse: that is off by one rounding of |lse| U and by the forward pass's ln s, 3 U
+    and 6 U of itself; log p takes one rounding more, its way to p two and an exponential 2 U.  p is off by that share of
+    itself: beside a p near 1, 1 - p has no more digits than |lse| U leaves it.  The sum with the one-hot term and the
+    products take four roundings."""
+    t, v, ranks = 40, 4096, 2
+    top = torch.randint(0, v, (t,), generator=torch.Generator().manual_seed(5))
+    wide = share * (0.7 + 0.6 * torch.rand(t, generator=torch.Generator().manual_seed(6)))
+    x = (most - ((v - 1) / wide).log())[:, None].expand(t, v).clone()
+    x[torch.arange(t), top] = most
+    g = rng_tensor(8, t)
+    w = worlds(ranks)
+    rows = Rows(x, DT.FP32, ranks)
+    _, lse, entropy, _, _ = rows.run(w, top)
+    got = grad_case(w, rows, top, 1.0, g, None, None, lse=lse, entropy=entropy)[0].double()
+    log_p = reference(rows.x, top, 1.0, 0)[5]
+    p, gd = log_p.exp(), g.double()[:, None]
+    exact = -p * gd
+    exact.scatter_add_(1, top[:, None], gd)
+    off = p * (abs(most) + 3 + 6 * share + 3 * log_p.abs() + 2) * U
+    assert bool(((got - exact).abs() <= (off + 4 * U * p) * gd.abs() + 4 * U * exact.abs()).all())
+
+
 def test_gradient_against_differences_of_the_forward_pass(worlds):
     """Central differences of the framework's own forward pass along random directions.  The loss is a sum of 4 log
     probabilities, 4 entropies and 8 alternatives with weights up to 3: every one is off by at most 400 U (V = 501), so a
