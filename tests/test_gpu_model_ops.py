@@ -1111,6 +1111,161 @@ def test_blocking_calls_from_one_thread_per_rank(worlds):
         w.close()
 
 
+def test_every_replay_writes_every_output(worlds):
+    """All four operators in one graph; before each replay every output, ids and gradients included, is overwritten and the
+    inputs are changed.  Each replay equals the eager calls on the same inputs, made in between on other buffers."""
+    if not torch.cuda.is_available():
+        pytest.skip("graphs need a GPU")
+    w = worlds(2)
+    many_tokens, few_tokens = given(1100, 300, 2).cuda(), given(3, 50001, 1).cuda()
+    weights = torch.ones(1100, device="cuda")
+    count = torch.ones(1, dtype=torch.int64, device="cuda")
+
+    class Buffers:
+        def __init__(self):
+            self.few = Rows(rng_tensor(1, 3, 50001), DT.BFP16, 2, 8)
+            self.many = Rows(rng_tensor(2, 1100, 300), DT.FP32, 2, 4)
+            self.grads = [torch.zeros_like(s) for s in self.many.shards]
+            self.tensor = Tensor(10007, (DT.BFP16, DT.BFP16, True), True, 4)
+            self.result = torch.zeros(2, 2, device="cuda")
+            self.size = model_ops.token_log_probs_workspace(3, 50001, 8)
+            self.space = torch.empty(self.size, dtype=torch.uint8, device="cuda")
+            self.norm_space = torch.empty(model_ops.grad_norm_workspace(2), dtype=torch.uint8, device="cuda")
+
+        def outputs(self):
+            return [o for rows in (self.few, self.many) for kind in (rows.log_probs, rows.lse, rows.entropy, rows.values, rows.ids)
+                    for o in kind] + self.grads + [self.result]
+
+        def restart(self, k):
+            """The inputs of step k; nothing left of an earlier one."""
+            for o in self.outputs():
+                o.fill_(77)
+            for rows in (self.few, self.many):
+                for s in rows.shards:
+                    s.copy_((rng_tensor(40 + k, s.shape[0], s.shape[1]) * 2).to(s.dtype))
+            for i, name in enumerate(sorted(self.tensor.rooms)):
+                view = self.tensor.view(name)
+                if view.dtype != torch.uint8:
+                    view.copy_((rng_tensor(60 + 10 * k + i, *view.shape).abs() * 0.01).to(view.dtype))
+                else:
+                    view.fill_(40 + k)
+
+        def step(self):
+            for rows, tokens, space in ((self.few, few_tokens, self.space), (self.many, many_tokens, None)):
+                with hccl_amd.group():
+                    for r, (start, n) in enumerate(rows.parts):
+                        s = rows.shards[r]
+                        model_ops.token_log_probs(
+                            w.comms[r], s, rows.t, start, n, tokens, rows.log_probs[r], data_type=rows.dtype,
+                            row_stride=s.stride(0), lse=rows.lse[r], entropy=rows.entropy[r], top_count=rows.top,
+                            top_values=rows.values[r], top_ids=rows.ids[r], workspace=space,
+                            workspace_bytes=self.size if space is not None else 0, stream=w.stream)
+            many = self.many
+            for r, (start, n) in enumerate(many.parts):
+                model_ops.token_log_probs_grad(
+                    w.comms[r], many.shards[r], 1100, start, n, many_tokens, many.lse[r], weights, self.grads[r],
+                    data_type=DT.FP32, row_stride=many.shards[r].stride(0), grad_row_stride=self.grads[r].stride(0),
+                    entropy=many.entropy[r], grad_entropy=weights, top_count=4, top_ids=many.ids[r],
+                    grad_top_values=many.values[r], stream=w.stream)
+            with hccl_amd.group():
+                for r in range(2):
+                    model_ops.grad_norm(w.comms[r], [(self.tensor.view("grad"), 10007, DT.BFP16)], 0.5, self.result[r],
+                                        workspace=self.norm_space, workspace_bytes=self.norm_space.numel(), stream=w.stream)
+            model_ops.adamw(w.comms[0], [self.tensor.descr()], 1, 1e-3, state_type=DT.FP8E4M3, clip=self.result[0],
+                            step_on_device=count, stream=w.stream)
+
+    kept, other = Buffers(), Buffers()
+    kept.restart(0)
+    torch.cuda.synchronize()
+    kept.step()      # (what is loaded at a first call is loaded)
+    w.sync()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=w.stream):
+        kept.step()
+    for k in range(1, 5):
+        for b in (kept, other):
+            b.restart(k)
+        few_tokens.add_(1)
+        many_tokens[7:].copy_(torch.randint(0, 300, (1093,), generator=torch.Generator().manual_seed(k)))
+        weights.copy_(rng_tensor(k, 1100))
+        count.fill_(k)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        other.step()
+        w.sync()
+        same = lambda a, b: torch.equal(a.float().nan_to_num(9e9), b.float().nan_to_num(9e9))  # noqa: E731
+        for i, (a, b) in enumerate(zip(kept.outputs(), other.outputs())):
+            assert same(a, b), (k, i)
+            assert bool((b != 77).any()), (k, i)
+        after, want = kept.tensor.host(), other.tensor.host()
+        for name in want:
+            assert same(after[name], want[name]), (k, name)
+        for rows in (kept.few, kept.many):      # against the definition, not only against another call
+            x = torch.cat([s[:, :n].cpu() for (_, n), s in zip(rows.parts, rows.shards)], 1)
+            tokens = (few_tokens if rows is kept.few else many_tokens).cpu()
+            part = Rows(x, rows.dtype, 2, rows.top, parts=rows.parts)
+            top = rows.top
+            check_rows(part, (rows.log_probs[1][:-1].cpu().double(), rows.lse[1][:-1].cpu().double(),
+                              rows.entropy[1][:-1].cpu().double(), rows.values[1][:-1].view(-1, top).cpu().double(),
+                              rows.ids[1][:-1].view(-1, top).cpu().long()), tokens, 1.0)
+
+
+@pytest.mark.parametrize("t,v", [(5, 3001), (3, 50001), (300, 700)])
+def test_threads_that_call_for_their_ranks_leave_every_output_right(worlds, t, v):
+    """A thread and a stream per rank, the inputs and every output replaced between two calls, rows shared by workgroups and
+    rows that are not: all of every rank's outputs afterwards, and all threads at their end."""
+    import threading
+    n, top = 3, 4
+    w = World(n)
+    try:
+        streams = [torch.cuda.Stream() for _ in range(n)]
+        size = max(16, model_ops.token_log_probs_workspace(t, v, top))
+        spaces = [torch.full((size,), 255, dtype=torch.uint8, device="cuda") for _ in range(n)]
+        norm_space = model_ops.grad_norm_workspace(n)
+        norm_spaces = [torch.full((norm_space,), 255, dtype=torch.uint8, device="cuda") for _ in range(n)]
+        for seed in range(3):
+            rows = Rows(rng_tensor(seed, t, v, scale=2.0), DT.FP32, n, top)
+            tokens = given(t, v, seed)
+            dev = tokens.cuda()
+            grads = [rng_tensor(seed + r, 1000 + r) for r in range(n)]
+            grads_dev = [g.cuda() for g in grads]
+            results = torch.full((n, 3), FILL, device="cuda")
+            errors = []
+            torch.cuda.synchronize()
+
+            def rank(r, rows=rows, dev=dev, grads_dev=grads_dev, results=results, errors=errors):
+                try:
+                    start, count = rows.parts[r]
+                    s = rows.shards[r]
+                    model_ops.token_log_probs(
+                        w.comms[r], s if count else None, t, start, count, dev, rows.log_probs[r], data_type=DT.FP32,
+                        row_stride=s.stride(0), lse=rows.lse[r], entropy=rows.entropy[r], top_count=top,
+                        top_values=rows.values[r], top_ids=rows.ids[r], workspace=spaces[r], workspace_bytes=size,
+                        stream=streams[r])
+                    model_ops.grad_norm(w.comms[r], [(grads_dev[r], 1000 + r, DT.FP32)], 1.0, results[r],
+                                        workspace=norm_spaces[r], workspace_bytes=norm_space, stream=streams[r])
+                except Exception as e:
+                    errors.append(e)
+            threads = [threading.Thread(target=rank, args=(r,), daemon=True) for r in range(n)]
+            for th in threads:
+                th.start()
+            for th in threads:
+                th.join(60)
+            assert not any(th.is_alive() for th in threads) and not errors, errors
+            torch.cuda.synchronize()
+            for r in range(n):
+                got = [o[r][:-1].cpu().double() for o in (rows.log_probs, rows.lse, rows.entropy, rows.values)]
+                check_rows(rows, (*got[:3], got[3].view(t, top), rows.ids[r][:-1].view(t, top).cpu().long()), tokens, 1.0)
+                assert all(float(o[r][-1]) == 77 for o in (rows.log_probs, rows.lse, rows.entropy, rows.values, rows.ids))
+            norm, factor = norm_reference([[(g, DT.FP32, 0)] for g in grads], 1.0, 1.0)
+            for r in range(n):
+                assert abs(float(results[r, 0]) - norm) <= 2 * U * norm and abs(float(results[r, 1]) - factor) <= 2 * U * factor
+            assert bool((results[:, 2] == FILL).all())
+    finally:
+        w.close()
+
+
 def test_a_sharded_training_step(worlds):
     """Two steps of a linear head, as the operators are used round the collectives: four ranks hold a quarter of the
     vocabulary's weights each and see the same rows (log probabilities and entropy over the split vocabulary, gradient of
