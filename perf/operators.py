@@ -9,7 +9,9 @@ Four operators that stand between a model and the collectives:
   adamw           one AdamW step over many tensors, with states in 32 bits or in FP8 blocks of 256
 
 `own` chooses between the plain form (elementary torch operations, 32 bits, 64 for long sums) and the calls a user
-makes of the framework.
+makes of the framework.  Those go to a stream of their own, as the library takes no null stream, and are ordered by the
+device alone: whoever calls `prepare` and `run` on another stream synchronizes the device between the two, before the
+results are read, and before a state is dropped.
 """
 import math
 import random
@@ -335,7 +337,8 @@ _worlds = {}
 
 
 def _world(ranks):
-    """The communicators of a world of that many ranks and the stream its calls go to, as a program keeps them."""
+    """The communicators of a world of that many ranks and the stream its calls go to, as a program keeps them.  (A program
+    that runs on that stream throughout needs no other order; events to and from the null stream take 35 us a pass.)"""
     import hccl_amd
     if ranks not in _worlds:
         _worlds[ranks] = (hccl_amd.comm_init_all(ranks), _worlds[min(_worlds)][1] if _worlds else torch.cuda.Stream())
