@@ -9,11 +9,12 @@
 // are then the bits that elementwise 32-bit operations give.  One bit more or less can decide between two codes, 6 %
 // apart, and one step later between two scales.  (With fused operations and the one-instruction root, four steps on 2^27
 // weights left 1371 codes and two scales that were not the same; 1 % faster with FP8 states, equally fast with 32-bit
-// ones.)  In the weights' step the reciprocal is the one-instruction form (1 ulp): it is 1e-7 of itself off, the weight far
-// less.  The root is not: that form takes a v below 2^-126 as 0, which would leave m / eps as a step.  (Equally fast.)
+// ones.)  In the weights' step the reciprocal, and with 32-bit states the root, are the one-instruction forms (1 ulp): it
+// is 1e-7 of itself off, the weight far less.  A v below 2^-126 is scaled for that root, which would be 0 and leave m / eps
+// as a step.  (630 us for the 2^27 weights below, with the correctly rounded root 635; 300 000 weights 5.0 with either.)
 //
 // Bound: every tensor read once and the updated ones written once.  2^27 bf16 weights in 300 tensors with 32-bit master
-// weights, four launches: 625 us, 6.0 TB/s of the 6.0 - 6.7 that a copy reaches; with FP8 states 381 us, 5.7 TB/s.  (A lane
+// weights, four launches: 630 us, 6.0 TB/s of the 6.0 - 6.7 that a copy reaches; with FP8 states 379 us, 5.7 TB/s.  (A lane
 // with eight neighbours, two 16-byte accesses 32 bytes apart: 790 and 486.  Chunks of 1024 elements 631 and 393, of 4096
 // 676 and 396; stores written through 651 and 391, plain ones 701 and 414.)
 #include "model_ops.h"
@@ -119,6 +120,13 @@ __device__ __forceinline__ void StoreCodes(uint64_t base, uint64_t at, uint32_t 
     }
 }
 
+// The root in one instruction (1 ulp), which takes what is below the smallest normal number as 0: that is scaled for it.
+__device__ __forceinline__ float Root(float v)
+{
+    const bool small = v < 0x1p-126f;
+    return __builtin_amdgcn_sqrtf(small ? v * 0x1p64f : v) * (small ? 0x1p-32f : 1.0f);
+}
+
 // Largest magnitude of a block.
 __device__ __forceinline__ float BlockMax(const float* x)
 {
@@ -203,7 +211,7 @@ __global__ __launch_bounds__(kThreads) void AdamWKernel(const AdamWArgs a)
             const float gi = g[s][i] * clip;
             m[s][i] = m[s][i] * a.beta1 + gi * a.oneMinusBeta1;
             v[s][i] = v[s][i] * a.beta2 + gi * gi * a.oneMinusBeta2;
-            root[i] = sqrtf(v[s][i]);
+            root[i] = kFp8 ? sqrtf(v[s][i]) : Root(v[s][i]);
             const float step = m[s][i] * __builtin_amdgcn_rcpf(__builtin_fmaf(root[i], rootCorrection2, a.eps));
             w[s][i] = __builtin_fmaf(-rate, step, w[s][i] * keep);
             if constexpr (kMaster) {
