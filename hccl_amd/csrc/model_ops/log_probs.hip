@@ -840,12 +840,27 @@ hipError_t Launch(LogProbsArgs& a, uint32_t rows, hipStream_t stream)
 //    512 x 131072   71.8 / 82.7     27.2 / 31.9     29.3 / 38.2     29.7 / 34.9 (2)
 //    256 x 32768    19.8 / 25.4      8.8 / 12.2      8.2 / 11.9      9.7 / 14.3 (2)
 //    256 x 131072   69.7 / 80.7     23.0 / 27.5     16.6 / 20.4     18.5 / 23.4 (4)
+//    255 x 131072                   22.7 / 27.4     16.6 / 20.4     18.1 / 23.5 (4)
+//    192 x 131072                   22.4 / 27.1     15.3 / 19.4     15.3 / 20.6 (4)
+//    129 x 131072                   21.7 / 26.4     14.5 / 18.7     14.2 / 19.5 (4)
+//    129 x 32768                     8.2 / 11.7      7.1 / 10.8      8.4 / 13.2 (4)
+//    192 x 16000                     6.9 / 9.8       7.5 / 11.2      8.6 / 12.7 (2)
 //    128 x 131072   68.4 / 80.0     21.8 / 26.6     14.5 / 18.6     12.6 / 17.7 (4)
 //     64 x 16000    10.4 / 14.1      6.2 / 8.9       7.0 / 10.3      7.1 / 11.5 (4)
 //     64 x 65536    35.4 / 42.5     12.4 / 16.4      9.0 / 13.0      8.2 / 12.7 (8)
 //     64 x 131072   67.6 / 78.7     21.4 / 25.9     14.0 / 18.3      9.7 / 14.6 (8)
 //     16 x 65536    29.2 / 34.2     11.2 / 14.1      8.7 / 12.2      6.7 / 11.0 (8)
 //      1 x 131072   46.0 / 55.6     14.3 / 18.4     12.0 / 15.7      6.1 / 10.6 (16)
+// With fp32 rows, whose vectors hold half as many:
+//   4096 x 16000    45.6 / 51.2     44.8 / 50.2     58.9 / 127      56.6 / 66.4 (2)
+//   1024 x 8000     11.9 / 15.5     10.4 / 13.6     16.2 / 32.3     14.5 / 20.6 (2)
+//    512 x 50001    46.1 / 53.7     19.8 / 23.8     21.8 / 31.1     23.9 / 28.6 (2)
+//    256 x 50001    44.4 / 51.6     16.6 / 20.8     13.6 / 17.1     15.6 / 20.4 (4)
+//    160 x 50001    43.8 / 51.3     15.9 / 19.9     10.8 / 14.2     12.5 / 17.3 (4)
+//     64 x 65536    52.7 / 61.8     17.4 / 21.9      9.9 / 13.4      8.9 / 13.4 (8)
+//     16 x 65536    43.8 / 51.0     15.3 / 19.3      9.3 / 12.7      7.4 / 11.5 (8)
+//      1 x 131072   77.6 / 85.4     25.2 / 29.1     13.6 / 17.0      6.1 / 10.4 (16)
+// fp16 rows take as long as bf16 in every form, or up to 7 % longer.
 // (Loading the next vectors before the present ones are summed: 4096 x 131072 175 against 174, 4096 x 16000 39 against 34,
 // 512 x 131072 25 against 27, with alternatives slower everywhere.  128 threads a row: 3 to 10 % faster than
 // the form taken for 2048 x 32000 and 16384 x 32000, up to 10 % slower for 4096 x 65536.)
