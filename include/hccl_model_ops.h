@@ -40,6 +40,7 @@ extern "C" {
  * its own.  -inf logits are entries that cannot occur.  A row of -inf alone has logSumExp -inf, logProbs -inf (0 if
  * ignored), entropy 0, topIds 0, 1, ... and topValues -inf.  A row with a NaN or +inf has NaN in every output but topIds,
  * which are -1, and the 0 of an ignored token.
+ * No output, and no workspace, may overlap anything else that the call reads or writes.
  */
 typedef struct {
     const void* logits;       /* tokenCount rows of vocabCount elements, rowStride elements apart, element-aligned */
