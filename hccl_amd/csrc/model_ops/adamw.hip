@@ -11,10 +11,11 @@
 // weights left 1371 codes and two scales that were not the same; 1 % faster with FP8 states, equally fast with 32-bit
 // ones.)  In the weights' step the reciprocal, and with 32-bit states the root, are the one-instruction forms (1 ulp): it
 // is 1e-7 of itself off, the weight far less.  A v below 2^-126 is scaled for that root, which would be 0 and leave m / eps
-// as a step.  (630 us for the 2^27 weights below, with the correctly rounded root 635; 300 000 weights 5.0 with either.)
+// as a step.  (With the correctly rounded root a call for 300 000 weights in 24 tensors
+// takes 6.5 us instead of 5.6, the 2^27 weights below as long.)
 //
 // Bound: every tensor read once and the updated ones written once.  2^27 bf16 weights in 300 tensors with 32-bit master
-// weights, four launches: 630 us, 6.0 TB/s of the 6.0 - 6.7 that a copy reaches; with FP8 states 379 us, 5.7 TB/s.  (A lane
+// weights, four launches: 632 us, 5.9 TB/s of the 6.0 - 6.7 that a copy reaches; with FP8 states 378 us, 5.7 TB/s.  (A lane
 // with eight neighbours, two 16-byte accesses 32 bytes apart: 790 and 486.  Chunks of 1024 elements 631 and 393, of 4096
 // 676 and 396; stores written through 651 and 391, plain ones 701 and 414.)
 #include "model_ops.h"
